@@ -77,7 +77,30 @@ EXPORTS = (
     "gnnagg_bf16_to_f32",
 )
 
+TRAIN_ABI_VERSION = 1   # GNNAGG_TRAIN_ABI_VERSION of include/gnn_train.h, the second header of the same library
+
+TRAIN_EXPORTS = (
+    "gnnagg_train_abi_version",
+    "gnnagg_rms_norm",
+    "gnnagg_rms_norm_fp8",
+    "gnnagg_rms_norm_backward_workspace_bytes",
+    "gnnagg_rms_norm_backward",
+    "gnnagg_fp8_quantize_rows",
+    "gnnagg_fp8_quantize_weight",
+    "gnnagg_fp8_product",
+    "gnnagg_fp8_weight_gradient_workspace_bytes",
+    "gnnagg_fp8_weight_gradient",
+    "gnnagg_adamw_step",
+)
+
 _lib = None
+
+
+class AdamwTensor(ctypes.Structure):
+    """``gnnagg_adamw_tensor`` of include/gnn_train.h."""
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
+                ("exp_avg_sq", ctypes.c_void_p), ("exp_avg_scales", ctypes.c_void_p),
+                ("exp_avg_sq_scales", ctypes.c_void_p), ("master", ctypes.c_void_p), ("n", ctypes.c_int64)]
 
 
 class PlanOptions(ctypes.Structure):
@@ -240,8 +263,43 @@ def lib() -> ctypes.CDLL:
     L.gnnagg_quantize_mixed_f32.argtypes = [vp, vp, vp, vp, i64, i64, vp, vp]
     L.gnnagg_dequantize_mixed_f32.restype = i32
     L.gnnagg_dequantize_mixed_f32.argtypes = [vp, vp, vp, vp, i64, i64, vp, vp]
+    _declare_train(L)
     _lib = L
     return L
+
+
+def _declare_train(L) -> None:
+    """Prototypes of include/gnn_train.h."""
+    vp, i64, i32, f64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_double
+    L.gnnagg_train_abi_version.restype = i32
+    L.gnnagg_train_abi_version.argtypes = []
+    built = L.gnnagg_train_abi_version()
+    if built != TRAIN_ABI_VERSION:
+        raise RuntimeError(f"{LIB_PATH} has training ABI version {built}, this binding was written against "
+                           f"{TRAIN_ABI_VERSION} (include/gnn_train.h changed since it was built): rebuild it "
+                           "(make -C gnn_benchmark_amd/csrc)")
+    L.gnnagg_rms_norm.restype = i32
+    L.gnnagg_rms_norm.argtypes = [vp, i64, vp, i64, vp, i32, f64, i32, vp, i64, vp, i64, i64, i64, i32, vp]
+    L.gnnagg_rms_norm_fp8.restype = i32
+    L.gnnagg_rms_norm_fp8.argtypes = [vp, i64, vp, i64, vp, i32, f64, i32, vp, i64, vp, vp, i64, i64, i32, vp]
+    L.gnnagg_rms_norm_backward_workspace_bytes.restype = i64
+    L.gnnagg_rms_norm_backward_workspace_bytes.argtypes = [i64, i64]
+    L.gnnagg_rms_norm_backward.restype = i32
+    L.gnnagg_rms_norm_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, i32, f64, i32, vp, i64, vp, vp, i64, i64, i64,
+                                           i32, vp]
+    L.gnnagg_fp8_quantize_rows.restype = i32
+    L.gnnagg_fp8_quantize_rows.argtypes = [vp, i64, vp, vp, i64, i64, i32, vp]
+    L.gnnagg_fp8_quantize_weight.restype = i32
+    L.gnnagg_fp8_quantize_weight.argtypes = [vp, i64, vp, vp, vp, i64, i64, i32, vp]
+    L.gnnagg_fp8_product.restype = i32
+    L.gnnagg_fp8_product.argtypes = [vp, vp, vp, vp, i64, i64, vp, vp, i64, i32, i64, i64, i64, vp]
+    L.gnnagg_fp8_weight_gradient_workspace_bytes.restype = i64
+    L.gnnagg_fp8_weight_gradient_workspace_bytes.argtypes = [i64, i64, i64]
+    L.gnnagg_fp8_weight_gradient.restype = i32
+    L.gnnagg_fp8_weight_gradient.argtypes = [vp, vp, vp, i64, i32, vp, vp, vp, i64, i64, i64, i64, vp]
+    L.gnnagg_adamw_step.restype = i32
+    L.gnnagg_adamw_step.argtypes = [ctypes.POINTER(AdamwTensor), i64, vp, i32, i32, i32, f64, vp, f64, f64, f64, f64,
+                                    ctypes.c_uint32, i64, vp]
 
 
 def check(rc: int) -> None:

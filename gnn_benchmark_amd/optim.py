@@ -1,0 +1,259 @@
+"""AdamW over many tensors at once, one launch for up to 48 of them, states in 32 or in 8 bits.
+
+``AdamW`` is a ``torch.optim.Optimizer`` for ``gcn.train_step`` / ``sage.train_step`` and any other loop;
+``adamw_step`` is the step on plain lists of tensors.  A step counts itself on the device, so it can be captured into a
+HIP graph and replayed.
+
+States in 8 bits are in the format of ``fp8`` (e4m3 codes, blocks of 128 elements, power-of-two scales): ``exp_avg`` is m
+rounded to nearest, ``exp_avg_sq`` holds sqrt(v) -- half the range in powers of two -- rounded to one of its two
+neighbours with the odds of the distance, because a step at ``beta2 = 0.999`` moves sqrt(v) by far less than half a code
+and rounding to nearest would never let it move.  The random bits come from a hash of (seed, tensor, step, element): the
+same calls give the same bits, on every rank.
+"""
+import ctypes
+from typing import List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+from .fp8 import BLOCK, dtype_code
+
+_FIELDS = 8  # words of a gnnagg_adamw_tensor
+
+
+def _same(tensors: Sequence[torch.Tensor], dtypes, device, what: str, count: int) -> torch.dtype:
+    if len(tensors) != count:
+        raise RuntimeError(f"Input mismatch: {len(tensors)} {what} for {count} parameters")
+    kinds = {t.dtype for t in tensors}
+    if len(kinds) != 1 or not kinds <= dtypes:
+        raise RuntimeError(f"Input mismatch: {what} must all have one type, of " + ", ".join(sorted(map(str, dtypes))))
+    for t in tensors:
+        if t.device != device:
+            raise RuntimeError(f"Input mismatch: {what} must be on the parameters' GPU (HIP) device, one is on {t.device}")
+        if not t.is_contiguous():
+            raise RuntimeError(f"Input mismatch: {what} must be contiguous")
+    return next(iter(kinds))
+
+
+_FLOATS = {torch.float32, torch.bfloat16}
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
+               exp_avg_sqs: Sequence[torch.Tensor], steps: torch.Tensor, *, lr: Union[float, torch.Tensor],
+               betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+               masters: Optional[Sequence[torch.Tensor]] = None,
+               exp_avg_scales: Optional[Sequence[torch.Tensor]] = None,
+               exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None, seed: int = 0, first: int = 0) -> None:
+    """One step in place: parameters, states and ``steps`` (int32 [len(params)], steps taken so far) are updated.
+
+    Parameters: all fp32, or all bf16 with fp32 ``masters`` (the values that are updated; the parameters receive them
+    rounded).  Gradients: all fp32 or all bf16.  States: fp32 ``exp_avgs`` / ``exp_avg_sqs``, or float8_e4m3fn codes of m
+    and sqrt(v) with ``exp_avg_scales`` / ``exp_avg_sq_scales`` (float8_e8m0fnu, one for each 128 elements).  ``lr``: a
+    number, or an fp32 scalar on the device that is read when the step runs.  ``first``: number of the first tensor for
+    the 8-bit states' random bits, where a list is split over calls."""
+    count = len(params)
+    if count == 0:
+        return
+    device = params[0].device
+    if device.type != "cuda":
+        raise RuntimeError("Input mismatch: parameters must be GPU (HIP) tensors")
+    with torch.no_grad():
+        param_dtype = _same(params, _FLOATS, device, "parameters", count)
+        grad_dtype = _same(grads, _FLOATS, device, "gradients", count)
+        state_dtype = _same(exp_avgs, {torch.float32, torch.float8_e4m3fn}, device, "states", count)
+        _same(exp_avg_sqs, {state_dtype}, device, "states", count)
+        lists = [params, grads, exp_avgs, exp_avg_sqs]
+        sizes = [p.numel() for p in params]
+        for tensors, what in ((grads, "gradient"), (exp_avgs, "state"), (exp_avg_sqs, "state")):
+            if [t.numel() for t in tensors] != sizes:
+                raise RuntimeError(f"Input mismatch: a {what} has another size than its parameter")
+        eight = state_dtype == torch.float8_e4m3fn
+        if eight:
+            if exp_avg_scales is None or exp_avg_sq_scales is None:
+                raise RuntimeError("Input mismatch: states in 8 bits need their scales")
+            blocks = [-(-n // BLOCK) for n in sizes]
+            for scales in (exp_avg_scales, exp_avg_sq_scales):
+                _same(scales, {torch.float8_e8m0fnu}, device, "scales", count)
+                if [t.numel() for t in scales] != blocks:
+                    raise RuntimeError("Input mismatch: scales hold one value for each 128 elements of their state")
+            lists += [exp_avg_scales, exp_avg_sq_scales]
+        elif exp_avg_scales is not None or exp_avg_sq_scales is not None:
+            raise RuntimeError("Input mismatch: states in 32 bits have no scales")
+        if param_dtype == torch.bfloat16:
+            if masters is None:
+                raise RuntimeError("Input mismatch: bfloat16 parameters need their float32 masters")
+            _same(masters, {torch.float32}, device, "masters", count)
+            if [t.numel() for t in masters] != sizes:
+                raise RuntimeError("Input mismatch: a master has another size than its parameter")
+        elif masters is not None:
+            raise RuntimeError("Input mismatch: float32 parameters have no masters")
+        if (steps.device != device or steps.dtype != torch.int32 or steps.dim() != 1 or steps.numel() != count
+                or not steps.is_contiguous()):
+            raise RuntimeError("Input mismatch: steps must be contiguous int32 [parameters] on their device")
+        lr_tensor = None
+        if isinstance(lr, torch.Tensor):
+            if lr.device == device:
+                if lr.dtype != torch.float32 or lr.numel() != 1:
+                    raise RuntimeError("Input mismatch: a learning rate on the device must be a float32 scalar")
+                lr_tensor, lr = lr, 0.0
+            else:
+                lr = float(lr)
+        records = (ctypes.c_uint64 * (_FIELDS * count))()
+        for at, tensors in enumerate(lists):
+            records[at::_FIELDS] = [t.data_ptr() for t in tensors]
+        if masters is not None:
+            records[6::_FIELDS] = [t.data_ptr() for t in masters]
+        records[7::_FIELDS] = sizes
+        with torch.cuda.device(device):
+            _lib.check(_lib.lib().gnnagg_adamw_step(
+                ctypes.cast(records, ctypes.POINTER(_lib.AdamwTensor)), count, _lib.ptr(steps),
+                dtype_code(param_dtype, "parameters"), dtype_code(grad_dtype, "gradients"), 8 if eight else 32, float(lr),
+                _lib.ptr(lr_tensor), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
+                int(seed) & 0xFFFFFFFF, int(first), _lib.current_stream(device)))
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW``'s update and arguments, each parameter group in a few launches.
+
+    ``state_bits`` 8 keeps both states of tensors of at least ``min_8bit_size`` elements in 8 bits (2 bytes an element
+    instead of 8), the others in 32.  bf16 parameters keep an fp32 master in their state.  A step can be captured into a
+    HIP graph once it has run eagerly (the states exist then); ``lr`` may be an fp32 scalar tensor on the device, which a
+    captured step reads anew at every replay.  Sparse gradients are refused."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits: int = 32,
+                 min_8bit_size: int = 4096, seed: int = 0):
+        if state_bits not in (32, 8):
+            raise ValueError("state_bits must be 32 or 8")
+        if not isinstance(lr, torch.Tensor) and lr < 0.0:
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"Invalid betas: {betas}")
+        if eps < 0.0 or weight_decay < 0.0:
+            raise ValueError("eps and weight_decay must not be negative")
+        self._runs = {}
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
+                                      state_bits=state_bits, min_8bit_size=min_8bit_size, seed=seed))
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._runs = {}
+
+    # ------------------------------------------------------------------ states
+    @staticmethod
+    def _kind(p: torch.Tensor, group) -> Tuple[torch.device, torch.dtype, int]:
+        bits = 8 if group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"] else 32
+        return p.device, p.dtype, bits
+
+    def _new_state(self, p: torch.Tensor, bits: int) -> dict:
+        if not p.is_cuda or p.dtype not in _FLOATS or not p.is_contiguous():
+            raise RuntimeError("Input mismatch: AdamW takes contiguous float32 or bfloat16 parameters on a GPU (HIP) device")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW's states do not exist yet: run one step before capturing one")
+        state = {}
+        flat = (p.numel(),)
+        if bits == 32:
+            for key in ("exp_avg", "exp_avg_sq"):
+                state[key] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        else:
+            for key in ("exp_avg", "exp_avg_sq"):
+                # the zero code and the scale byte of an empty block
+                state[key] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
+                state[key + "_scales"] = torch.ones(-(-flat[0] // BLOCK), dtype=torch.uint8,
+                                                    device=p.device).view(torch.float8_e8m0fnu)
+        if p.dtype == torch.bfloat16:
+            state["master"] = p.detach().float()
+        return state
+
+    def _prepare(self, index: int, group) -> list:
+        """The group's parameters in an order that puts those of one kind (device, type, state) side by side, with one
+        array of step counts for each kind: [(kind, parameters, steps)].  ``state[p]["step"]`` is p's entry of it."""
+        runs = self._runs.get(index)
+        if runs is not None and sum(len(ps) for _, ps, _ in runs) == len(group["params"]):
+            return runs
+        kinds = {}
+        for p in group["params"]:
+            kinds.setdefault(self._kind(p, group), []).append(p)
+        runs = []
+        for kind, ps in kinds.items():
+            taken = [self.state[p].get("step", 0) if p in self.state else 0 for p in ps]
+            if kind[0].type != "cuda":
+                raise RuntimeError("Input mismatch: AdamW takes parameters on a GPU (HIP) device")
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW's states do not exist yet: run one step before capturing one")
+            steps = torch.tensor([int(t) for t in taken], dtype=torch.int32, device=kind[0])
+            for i, p in enumerate(ps):
+                if p in self.state and self.state[p]:
+                    self.state[p]["step"] = steps[i]
+            runs.append((kind, ps, steps))
+        self._runs[index] = runs
+        return runs
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for index, group in enumerate(self.param_groups):
+            number = 0
+            for (_, _, bits), ps, steps in self._prepare(index, group):
+                at = 0
+                while at < len(ps):  # stretches of parameters that have a gradient: each has its own count of steps
+                    if ps[at].grad is None:
+                        at += 1
+                        continue
+                    end = at
+                    while end < len(ps) and ps[end].grad is not None:
+                        end += 1
+                    self._step_stretch(group, ps[at:end], steps, at, bits, number + at)
+                    at = end
+                number += len(ps)
+        return loss
+
+    def _step_stretch(self, group, ps: List[torch.Tensor], steps, at: int, bits: int, number: int) -> None:
+        states = []
+        for i, p in enumerate(ps):
+            if p.grad.is_sparse:
+                raise RuntimeError("AdamW does not take sparse gradients")
+            state = self.state[p]
+            if not state:
+                state.update(self._new_state(p, bits))
+                state["step"] = steps[at + i]
+            states.append(state)
+        grads = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in ps]
+        adamw_step(ps, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], steps[at:at + len(ps)],
+                   lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                   masters=[s["master"] for s in states] if ps[0].dtype == torch.bfloat16 else None,
+                   exp_avg_scales=[s["exp_avg_scales"] for s in states] if bits == 8 else None,
+                   exp_avg_sq_scales=[s["exp_avg_sq_scales"] for s in states] if bits == 8 else None,
+                   seed=group["seed"], first=number)
+
+    # ------------------------------------------------------------------ checkpoints
+    def load_state_dict(self, state_dict) -> None:
+        """Takes over a ``state_dict`` of this class, or one of ``torch.optim.Adam`` / ``AdamW`` with fp32 states where
+        this optimizer's states are in 32 bits.  (torch's own loading casts states to their parameter's type, which
+        would turn 8-bit codes and fp32 states of bf16 parameters into something else.)"""
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        keep = ("state_bits", "min_8bit_size", "seed")
+        groups = []
+        for g, own in zip(state_dict["param_groups"], self.param_groups):
+            groups.append({**{k: own[k] for k in keep}, **{k: v for k, v in g.items()}})
+        super().load_state_dict({"state": {}, "param_groups": groups if len(groups) == len(state_dict["param_groups"])
+                                 else state_dict["param_groups"]})
+        own = [(p, g) for g in self.param_groups for p in g["params"]]
+        for i, (p, group) in zip(saved, own):
+            old = state_dict["state"].get(i)
+            if not old:
+                continue
+            state = self._new_state(p, self._kind(p, group)[2])
+            for key, t in state.items():
+                src = old.get(key)
+                if key == "master" and src is None:
+                    continue
+                if src is None or src.dtype != t.dtype or src.shape != t.shape:
+                    raise RuntimeError(f"Input mismatch: the saved {key} does not fit this optimizer's states (type and "
+                                       "shape have to be the same)")
+                t.copy_(src)
+            state["step"] = int(old["step"])
+            self.state[p] = state
+        self._runs = {}
