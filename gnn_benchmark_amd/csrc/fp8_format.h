@@ -141,6 +141,13 @@ __device__ __forceinline__ f32x4 rounded(const bf16_t *, const f32x4 v) {
 // way to registers, which takes the point out of asking for them early.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// keeps an address that is the same for the whole wave in scalar registers
+template <typename T>
+__device__ __forceinline__ const T *scalar(const T *p) {
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
 // host: may rows at p with this stride and width be moved four values at a time?
 inline bool vec4_rows(const void *p, int64_t stride, int64_t width, int dtype) {
     const uintptr_t bytes = dtype == GNNAGG_F32 ? 16 : 8;

@@ -13,14 +13,17 @@
 //          their way from LDS into the matrix unit -- and multiply on v_mfma_f32_*_bf16: every product exact, sums fp32
 //          (2e-8 off on the same operands), at half the matrix rate.
 //
-// Both operands have the contraction index contiguous, 128 codes = 128 bytes a block, so one pipeline stage is one block: a 128-byte piece of every row of
-// the tile, copied straight from global memory into LDS (no registers between), double-buffered, one barrier a stage.
+// Both operands have the contraction index contiguous.  A pipeline stage is half a block of it, 64 bytes of every row of the
+// tile, copied straight from global memory into one of four LDS buffers (no registers between), three stages ahead of the
+// matrix unit; one barrier a stage.
 //
 // w is the MFMA's first operand: a lane then owns runs of four consecutive columns of one row of the result.
 //
-// The 16-byte pieces of a staged row are stored at piece ^ ((row / 2) % 8): the 16 lanes of a ds_read_b128 phase read the
-// same piece of 16 neighbouring rows, and two rows fill the 64 banks, so every phase touches each bank once.
+// The 16-byte pieces of a staged row are stored at piece ^ ((row / 4) % 4).  A 16-byte LDS access takes its lanes in fours
+// of which groups 0, 3, 5, 6 (and 1, 2, 4, 7) of a half-wave go together; four rows fill the banks once, and with this order
+// such 16 lanes, reading the same piece of their rows, touch every bank once.
 #include <type_traits>
+
 
 #include "fp8_format.h"
 
@@ -70,6 +73,18 @@ __device__ __forceinline__ bf16x8_t decode8(int lo, int hi, float power) {
 }
 __device__ __forceinline__ float scale_value(int byte) { return __uint_as_float((uint32_t)byte << 23); }
 
+typedef uint32_t unaligned_word __attribute__((aligned(1)));
+
+// This wave's LDS reads are done and so are its loads and copies but the YOUNGEST ones; and so are everybody's.  (The wait
+// is a builtin that the compiler counts: it waits for none of these again.)
+template <int YOUNGEST>
+__device__ __forceinline__ void landed() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((YOUNGEST & 15) | (YOUNGEST >> 4) << 14 | 0x70);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // block number -> tile number: the blocks of one XCD (every eighth) take a stretch of neighbouring tiles
 __device__ __forceinline__ int64_t tile_of(int64_t block, int64_t tiles) {
     const int64_t q = tiles / 8, r = tiles % 8, xcd = block % 8, i = block / 8;
@@ -91,49 +106,74 @@ __global__ __launch_bounds__(64 * MW * NW) void fp8_product_kernel(const Product
     constexpr bool kExact = sizeof(O) == 4;
     constexpr int kWaves = MW * NW;
     constexpr int kM = 32 * WM * MW, kN = 32 * WN * NW;
-    constexpr int kCopies = (kM + kN) / 8 / kWaves;   // copies of 8 rows a wave and stage
-    static_assert((kM + kN) % (8 * kWaves) == 0 && 32 * WN <= kBlock8, "");
-    extern __shared__ __align__(128) uint8_t lds[];   // two stages of (kM + kN) rows of 128 bytes
-    constexpr int kStage = (kM + kN) * kBlock8;
+    constexpr int kHalf = kBlock8 / 2;                  // bytes of a row in a stage
+    constexpr int kCopies = (kM + kN) / 16 / kWaves;    // copies of 16 rows a wave and stage
+    static_assert((kM + kN) % (16 * kWaves) == 0 && 32 * WN <= kBlock8, "");
+    extern __shared__ __align__(128) uint8_t lds[];     // four stages of (kM + kN) rows
+    constexpr int kStage = (kM + kN) * kHalf;
 
     const int lane = (int)threadIdx.x % 64;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
     const int wm = wave / NW, wn = wave % NW;
     const int idx = lane % 32, half = lane / 32;
-    const int64_t tiles_n = (p.n + kN - 1) / kN;
+    // neighbouring tiles: eight down, then the next column, so that the tiles at work on one XCD share both operands
+    const int64_t tiles_n = (p.n + kN - 1) / kN, tiles_m = (p.rows + kM - 1) / kM;
     const int64_t tile = tile_of(blockIdx.x, gridDim.x);
-    const int64_t m0 = tile / tiles_n * kM, n0 = tile % tiles_n * kN;
+    const int64_t band = tile / (8 * tiles_n), in_band = tile - band * 8 * tiles_n;
+    const int64_t high = tiles_m - 8 * band < 8 ? tiles_m - 8 * band : 8;
+    const int64_t m0 = (8 * band + in_band % high) * kM, n0 = in_band / high * kN;
     const int64_t pitch = (int64_t)p.blocks * kBlock8;
 
-    // what this lane copies: rows past the end read the last row, their results are never stored
-    const uint8_t *src[kCopies];
+    // what this lane copies, from the tile's first row on: rows past the end read the last row, their results are never
+    // stored
+    const uint8_t *x_tile = p.x + m0 * pitch, *w_tile = p.w + n0 * pitch;
+    uint32_t src[kCopies];
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
-        const int row = (wave * kCopies + i) * 8 + lane / 8;
-        const int piece = (lane % 8) ^ ((row / 2) % 8);
+        const int row = (wave * kCopies + i) * 16 + lane / 4;
+        const int piece = (lane % 4) ^ ((row / 4) % 4);
         const bool is_x = row < kM;
-        int64_t r = is_x ? m0 + row : n0 + (row - kM);
-        const int64_t last = (is_x ? p.rows : p.n) - 1;
-        r = r < last ? r : last;
-        src[i] = (is_x ? p.x : p.w) + r * pitch + 16 * piece;
+        const int64_t last = (is_x ? p.rows - m0 : p.n - n0) - 1;
+        const int r = is_x ? row : row - kM;
+        src[i] = (uint32_t)((r < last ? r : last) * pitch) + 16 * piece;
     }
-    auto fetch = [&](int stage, int block) {
+    auto fetch = [&](int stage, int from, int to) {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i)
-            copy_to_lds(src[i] + (int64_t)block * kBlock8, lds + stage * kStage + (wave * kCopies + i) * 8 * kBlock8);
+            if (i >= from && i < to) {
+                const int row = (wave * kCopies + i) * 16;  // (a copy's rows are all x's or all w's)
+                copy_to_lds(scalar((row < kM ? x_tile : w_tile) + (int64_t)stage * kHalf) + src[i],
+                            lds + stage % 4 * kStage + row * kHalf);
+            }
     };
 
+    // A lane's scales of x: the bytes of four neighbouring blocks of its row in one (unaligned) word, for each fragment --
+    // a byte for each block costs a cache line a lane and block, which took a quarter of the time (8192^3: 659 us against
+    // 484 without them).  A word that would end past the array is read where the array ends, and shifted.
+    const int64_t wm0 = m0 + wm * 32 * WM;
     const uint8_t *xs[WM];
-    int64_t wm0 = m0 + wm * 32 * WM;
+    int beyond[WM];                   // blocks from which on the word would end past the array
 #pragma unroll
     for (int i = 0; i < WM; ++i) {
         int64_t m = wm0 + 32 * i + idx;
         m = m < p.rows ? m : p.rows - 1;
         xs[i] = p.x_scales + m * p.blocks;
+        const int64_t room = (p.rows - m) * p.blocks - 4;
+        beyond[i] = room < p.blocks ? (int)room : p.blocks;
     }
     const int64_t wn0 = n0 + wn * 32 * WN;
     const int64_t nb = (wn0 < p.n ? wn0 : p.n - 1) / kBlock8;
     const uint8_t *ws = p.w_scales + nb * p.scale_n_stride;
+    uint32_t four[WM];                // x's scales of the group of four blocks at work, the first block's in the low byte
+    int w_next;                       // w's scale of the next block
+    auto load_four = [&](int block) {
+#pragma unroll
+        for (int i = 0; i < WM; ++i)
+            four[i] = *reinterpret_cast<const unaligned_word *>(xs[i] + (block < beyond[i] ? block : beyond[i]));
+    };
+    struct Scales {
+        int x[WM], w;
+    };
 
     f32x16 acc[WM][WN];
 #pragma unroll
@@ -143,74 +183,107 @@ __global__ __launch_bounds__(64 * MW * NW) void fp8_product_kernel(const Product
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-    // byte offsets of a lane's four 16-byte pieces in a staged row of its fragment
-    int piece_off[4];
+    // byte offsets of a lane's two 16-byte pieces in a staged row of its fragment
+    int piece_off[2];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) piece_off[q] = idx * kBlock8 + 16 * (((q / 2) * 4 + half * 2 + q % 2) ^ ((idx / 2) % 8));
-
-    fetch(0, 0);
-    int sx[WM], sw;
+    for (int q = 0; q < 2; ++q) piece_off[q] = idx * kHalf + 16 * ((2 * half + q) ^ ((idx / 4) % 4));
+    constexpr int kPieces = 2 * (WM + WN);
+    struct Fragments {
+        i32x4 piece[kPieces];  // w's, then x's, two 16-byte pieces each
+        __device__ __forceinline__ i32x8 get(int f) const {
+            return __builtin_shufflevector(piece[2 * f], piece[2 * f + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    };
+    auto read = [&](Fragments &f, int stage, int from, int to) {
+        const uint8_t *at = lds + stage % 4 * kStage;
+        const uint8_t *xt = at + wm * 32 * WM * kHalf, *wt = at + (kM + wn * 32 * WN) * kHalf;
 #pragma unroll
-    for (int i = 0; i < WM; ++i) sx[i] = xs[i][0];
-    sw = ws[0];
-    for (int b = 0; b < p.blocks; ++b) {
-        // this stage has landed (every wave waits for its own copies), and everybody is done with the other one
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        const uint8_t *stage = lds + (b & 1) * kStage;
-        int nx[WM], nw = 0;
-        const int next = b + 1 < p.blocks ? b + 1 : b;
-        if (b + 1 < p.blocks) fetch((b + 1) & 1, b + 1);
+        for (int r = 0; r < kPieces; ++r)
+            if (r >= from && r < to)
+                f.piece[r] = *reinterpret_cast<const i32x4 *>((r < 2 * WN ? wt + 32 * (r / 2) * kHalf : xt + 32 * (r / 2 - WN) * kHalf) +
+                                                              piece_off[r % 2]);
+    };
+    // Multiplies a stage.  `beside(q)` is called behind the q-th matrix instruction; the empty statement that names the
+    // sum keeps the instruction in front of it.
+    constexpr int kSteps = (kExact ? 4 : 1) * WM * WN;
+    auto multiply = [&](const Fragments &f, const Scales &s, auto beside) {
+        if constexpr (!kExact) {
 #pragma unroll
-        for (int i = 0; i < WM; ++i) nx[i] = xs[i][next];
-        nw = ws[next * p.scale_k_stride];
-        const uint8_t *xt = stage + wm * 32 * WM * kBlock8, *wt = stage + (kM + wn * 32 * WN) * kBlock8;
+            for (int i = 0; i < WM; ++i)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            i32x8 fx[WM], fw[WN];
+                for (int j = 0; j < WN; ++j) {
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f.get(j), f.get(WN + i), acc[i][j], 0, 0, 0, s.w, 0, s.x[i]);
+                    asm volatile("" : "+a"(acc[i][j]));
+                    beside(i * WN + j);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        } else {
+            // a lane's codes eight at a time: the contraction in another order, the same for both operands
 #pragma unroll
-            for (int j = 0; j < WN; ++j) {
-                const i32x4 lo = *reinterpret_cast<const i32x4 *>(wt + 32 * j * kBlock8 + piece_off[2 * s]);
-                const i32x4 hi = *reinterpret_cast<const i32x4 *>(wt + 32 * j * kBlock8 + piece_off[2 * s + 1]);
-                fw[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
+            for (int t = 0; t < 4; ++t) {
+                bf16x8_t hw[WN];
 #pragma unroll
-            for (int i = 0; i < WM; ++i) {
-                const i32x4 lo = *reinterpret_cast<const i32x4 *>(xt + 32 * i * kBlock8 + piece_off[2 * s]);
-                const i32x4 hi = *reinterpret_cast<const i32x4 *>(xt + 32 * i * kBlock8 + piece_off[2 * s + 1]);
-                fx[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
-            if constexpr (!kExact) {
+                for (int j = 0; j < WN; ++j)
+                    hw[j] = decode8(f.piece[2 * j + t / 2][2 * (t % 2)], f.piece[2 * j + t / 2][2 * (t % 2) + 1], scale_value(s.w));
 #pragma unroll
-                for (int i = 0; i < WM; ++i)
+                for (int i = 0; i < WM; ++i) {
+                    const i32x4 c = f.piece[2 * (WN + i) + t / 2];
+                    const bf16x8_t hx = decode8(c[2 * (t % 2)], c[2 * (t % 2) + 1], scale_value(s.x[i]));
 #pragma unroll
-                    for (int j = 0; j < WN; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[j], fx[i], acc[i][j], 0, 0, 0, sw, 0, sx[i]);
-            } else {
-                // a lane's codes eight at a time: the contraction in another order, the same for both operands
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    bf16x8_t hw[WN];
-#pragma unroll
-                    for (int j = 0; j < WN; ++j) hw[j] = decode8(fw[j][2 * t], fw[j][2 * t + 1], scale_value(sw));
-#pragma unroll
-                    for (int i = 0; i < WM; ++i) {
-                        const bf16x8_t hx = decode8(fx[i][2 * t], fx[i][2 * t + 1], scale_value(sx[i]));
-#pragma unroll
-                        for (int j = 0; j < WN; ++j)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hw[j], hx, acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < WN; ++j) {
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hw[j], hx, acc[i][j], 0, 0, 0);
+                        asm volatile("" : "+a"(acc[i][j]));
+                        beside((t * WM + i) * WN + j);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
+    };
+
+    // Stage s is multiplied out of registers while s + 1 is read from LDS and s + 4 is sent for into the buffer that s was
+    // read from.  Reads and copies are dealt out among the matrix instructions: sent at once they fill their queues and the
+    // wave waits in front of its products.
+    Fragments f[2];
+    auto step = [&](int s, auto part, const Scales &now, bool more) {
+        constexpr int q0 = decltype(part)::value;
+        multiply(f[q0], now, [&](int q) {
+            read(f[1 - q0], s + 1, 2 * q * kPieces / kSteps, 2 * (q + 1) * kPieces / kSteps);  // (behind the last stage:
+            if (more) fetch(s + 4, q * kCopies / kSteps, (q + 1) * kCopies / kSteps);          //  what its buffer held)
+        });
+    };
+    const std::integral_constant<int, 0> first;
+    const std::integral_constant<int, 1> second;
+    auto block = [&](int b, auto more) {
+        constexpr bool kMore = decltype(more)::value;
+        landed<kMore ? 2 * kCopies : 0>();  // the copies of stages 2 b + 2 and 2 b + 3 may be on their way
+        Scales now;
 #pragma unroll
         for (int i = 0; i < WM; ++i) {
-            sx[i] = nx[i];
-            asm volatile("" : "+v"(sx[i]));  // (the next block's scales are loaded behind this one's products, not
-        }                                    //  sunk to their first use)
-        sw = nw;
-        asm volatile("" : "+v"(sw));
+            const int at = (b & ~3) < beyond[i] ? b & ~3 : beyond[i];  // the first block in the word
+            now.x[i] = (int)(four[i] >> (8 * (b - at)));               // (the low byte counts)
+            if constexpr (kExact) now.x[i] &= 0xff;
+        }
+        now.w = w_next;
+        if (b % 4 == 3 && b + 1 < p.blocks) load_four(b + 1);
+        w_next = ws[(b + 1 < p.blocks ? b + 1 : b) * p.scale_k_stride];
+        step(2 * b, first, now, kMore);
+        landed<kMore ? 2 * kCopies : 0>();
+        step(2 * b + 1, second, now, kMore);
+    };
+    fetch(0, 0, kCopies);
+    load_four(0);
+    w_next = ws[0];
+    landed<0>();
+    fetch(1, 0, kCopies);
+    if (p.blocks > 1) {
+        fetch(2, 0, kCopies);
+        fetch(3, 0, kCopies);
     }
+    read(f[0], 0, 0, kPieces);
+    int b = 0;
+    for (; b + 2 < p.blocks; ++b) block(b, std::true_type());
+    for (; b < p.blocks; ++b) block(b, std::false_type());
 
     // register r of lane l holds column (r % 4) + 8 (r / 4) + 4 (l / 32) of the tile, row l % 32
 #pragma unroll
@@ -226,6 +299,136 @@ __global__ __launch_bounds__(64 * MW * NW) void fp8_product_kernel(const Product
                 const f32x4 v = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]} + b4;
                 store_run(static_cast<O *>(p.out) + m * p.out_stride, c, p.n, p.vec, v);
             }
+        }
+    }
+}
+
+// Many rows against a small weight (a layer of a graph's nodes): bound by x's and the result's bytes.  The whole weight stays
+// in LDS, a persistent block a compute unit; its eight waves then work apart, with no barrier, each on 32 rows at a time
+// whose codes it reads straight into registers, so that one wave's loads and stores run beside another's products
+// (1 M x 512 x 256 to fp32: 0.40 ms = 3.8 TB/s; the tiled kernel, whose blocks live for eight short stages there: 0.64 ms).
+// x is the first operand here: a lane holds one column of each of four tiles of 32 x 32, and as tile j takes the weight's rows
+// 4 i + j, the four are neighbours in the result: 16 bytes a lane, 512 bytes a row in one store.  Rows of the weight lie
+// in that order, 16 bytes further apart than they are long: 16 neighbouring ones start on 16 different groups of banks.
+template <typename O, int KB>
+__global__ __launch_bounds__(512, 2) void fp8_product_rows_kernel(const ProductArgs p) {
+    constexpr bool kExact = sizeof(O) == 4;
+    constexpr int kStages = 2 * KB;                       // of 64 along the contraction
+    constexpr int kPitch = KB * kBlock8 + 16;
+    extern __shared__ __align__(128) uint8_t lds[];       // the weight, then its scales [groups][KB]
+    const int lane = (int)threadIdx.x % 64, idx = lane % 32, half = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+    const int groups = (int)((p.n + kBlock8 - 1) / kBlock8);
+    uint8_t *w_scales = lds + groups * kBlock8 * kPitch;
+
+    // row n of the weight -> place 128 (n / 128) + 32 (n % 4) + n % 128 / 4; places without a row stay as they are, their
+    // results are not stored.  A thread keeps to one piece of the row (512 threads are 64 / KB rows), eight in flight.
+    constexpr int kRowPieces = 8 * KB, kRowsAtOnce = 512 / kRowPieces;
+    const int q = (int)threadIdx.x % kRowPieces;
+    if ((int)threadIdx.x < kRowsAtOnce * kRowPieces) {
+        const uint8_t *src = p.w + 16 * q;
+        for (int n0 = (int)threadIdx.x / kRowPieces; n0 < p.n; n0 += 8 * kRowsAtOnce) {
+            i32x4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int n = n0 + u * kRowsAtOnce;
+                v[u] = *reinterpret_cast<const i32x4 *>(src + (int64_t)(n < p.n ? n : (int)p.n - 1) * (KB * kBlock8));
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int n = n0 + u * kRowsAtOnce;
+                if (n < p.n)
+                    *reinterpret_cast<i32x4 *>(lds + ((n & ~127) + 32 * (n & 3) + ((n & 127) >> 2)) * kPitch + 16 * q) = v[u];
+            }
+        }
+    }
+    for (int i = threadIdx.x; i < groups * KB; i += 512)
+        w_scales[i] = p.w_scales[(i % KB) * p.scale_k_stride + (i / KB) * p.scale_n_stride];
+    __syncthreads();
+
+    const int64_t tiles = (p.rows + 31) / 32, stride = (int64_t)gridDim.x * 8;
+    i32x4 x[kStages][2];
+    int sx[KB];
+    auto load = [&](int64_t tile) {
+        int64_t m = tile * 32 + idx;
+        m = m < p.rows ? m : p.rows - 1;
+        // a stage's four pieces of a row go to the two lanes that have it in turn (w's too: any order of the contraction
+        // will do)
+        const uint8_t *row = p.x + m * (KB * kBlock8) + 16 * half;
+#pragma unroll
+        for (int s = 0; s < kStages; ++s) {
+            x[s][0] = *reinterpret_cast<const i32x4 *>(row + 64 * s);
+            x[s][1] = *reinterpret_cast<const i32x4 *>(row + 64 * s + 32);
+        }
+#pragma unroll
+        for (int b = 0; b < KB; ++b) sx[b] = p.x_scales[m * KB + b];
+    };
+    f32x16 acc[4];
+    auto multiply = [&](int g) {
+        if constexpr (!kExact) asm volatile("" ::: "memory");  // (the weight does not change: without this its reads are
+#pragma unroll                                                 //  hoisted out of the loop over tiles, and spilled)
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[j][r] = 0.0f;
+        const uint8_t *wt = lds + (g * kBlock8 + idx) * kPitch + 16 * half;
+        i32x4 w[2][4][2];                                 // a stage's, and the next one's on its way from LDS
+        auto read = [&](int s) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[s % 2][j][0] = *reinterpret_cast<const i32x4 *>(wt + 32 * j * kPitch + 64 * s);
+                w[s % 2][j][1] = *reinterpret_cast<const i32x4 *>(wt + 32 * j * kPitch + 64 * s + 32);
+            }
+        };
+        if constexpr (!kExact) read(0);
+#pragma unroll
+        for (int s = 0; s < kStages; ++s) {
+            const int sw = w_scales[g * KB + s / 2];
+            const auto &ws = w[s % 2];
+            if constexpr (!kExact) {
+                if (s + 1 < kStages) read(s + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                        __builtin_shufflevector(x[s][0], x[s][1], 0, 1, 2, 3, 4, 5, 6, 7),
+                        __builtin_shufflevector(ws[j][0], ws[j][1], 0, 1, 2, 3, 4, 5, 6, 7), acc[j], 0, 0, 0, sx[s / 2], 0, sw);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(acc[j]));  // (keeps the stages apart)
+                __builtin_amdgcn_sched_barrier(0);
+            } else {                                      // (decoding leaves no room for a second stage of w)
+                read(s);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const bf16x8_t hx = decode8(x[s][t / 2][2 * (t % 2)], x[s][t / 2][2 * (t % 2) + 1], scale_value(sx[s / 2]));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            hx, decode8(ws[j][t / 2][2 * (t % 2)], ws[j][t / 2][2 * (t % 2) + 1], scale_value(sw)), acc[j], 0, 0, 0);
+                }
+            }
+        }
+    };
+    // register r of lane l holds row (r % 4) + 8 (r / 4) + 4 (l / 32) of the tile, column l % 32 of tile j
+    auto store = [&](int64_t tile, int g) {
+        const int64_t c = (int64_t)g * kBlock8 + 4 * idx;
+        const f32x4 b4 = p.bias ? load4<false>(p.bias, c, p.n) : f32x4{0.f, 0.f, 0.f, 0.f};
+        O *out = static_cast<O *>(p.out) + (tile * 32 + 4 * half) * p.out_stride;
+        const bool whole = tile * 32 + 32 <= p.rows;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int row = r % 4 + 8 * (r / 4);
+            if (!whole && tile * 32 + 4 * half + row >= p.rows) continue;
+            const f32x4 v = f32x4{acc[0][r], acc[1][r], acc[2][r], acc[3][r]} + b4;
+            store_run(out + row * p.out_stride, c, p.n, p.vec, v);
+        }
+    };
+    int64_t tile = (int64_t)wave * gridDim.x + blockIdx.x;
+    if (tile < tiles) load(tile);
+    for (; tile < tiles; tile += stride) {
+        for (int g = 0; g < groups; ++g) {
+            multiply(g);
+            if (g == groups - 1) load(tile + stride);  // in front of the stores
+            store(tile, g);
         }
     }
 }
@@ -294,7 +497,7 @@ __global__ __launch_bounds__(512) void fp8_product_few_kernel(const ProductArgs 
 template <typename O, int WM, int WN, int MW, int NW>
 int launch_tiles(const ProductArgs &p, hipStream_t st) {
     constexpr int kM = 32 * WM * MW, kN = 32 * WN * NW;
-    constexpr size_t kLds = 2 * (size_t)(kM + kN) * kBlock8;
+    constexpr size_t kLds = 4 * (size_t)(kM + kN) * (kBlock8 / 2);
     const int64_t tiles = ((p.rows + kM - 1) / kM) * ((p.n + kN - 1) / kN);
     if (tiles > 0x7fffffff) return fail(GNNAGG_ERR_UNSUPPORTED, "too many tiles");
     auto kernel = fp8_product_kernel<O, WM, WN, MW, NW>;
@@ -305,10 +508,31 @@ int launch_tiles(const ProductArgs &p, hipStream_t st) {
     return GNNAGG_OK;
 }
 
+// LDS of the kernel that keeps the weight there; 0: it does not fit
+inline size_t rows_lds(const ProductArgs &p) {
+    if (p.blocks > 4) return 0;
+    const size_t groups = (size_t)((p.n + kBlock8 - 1) / kBlock8);
+    const size_t bytes = groups * kBlock8 * (p.blocks * kBlock8 + 16) + groups * p.blocks;
+    return p.n <= 4096 && bytes <= 160 * 1024 ? bytes : 0;
+}
+
+template <typename O, int KB>
+int launch_rows(const ProductArgs &p, hipStream_t st) {
+    auto kernel = fp8_product_rows_kernel<O, KB>;
+    const size_t bytes = rows_lds(p);
+    GNNAGG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    hipLaunchKernelGGL(kernel, dim3(256), dim3(512), bytes, st, p);
+    GNNAGG_HIP(hipGetLastError());
+    return GNNAGG_OK;
+}
+
 template <typename O>
 int launch_product(const ProductArgs &p, hipStream_t st) {
     const int64_t columns = (p.n + 15) / 16;
-    if (p.rows <= 64) {
+    // Few rows, or a small result: the tiled kernel would have a block for each 128 columns and rows only, this one has one
+    // for each 16 columns and 64 rows (to fp32, this kernel / tiles: 65 x 1024 x 1024 5 / 13 us, 300 x 512 x 256 4 / 9 us,
+    // 128 x 4096 x 4096, two blocks a compute unit, 28 / 36 us, 300 x 4096 x 4096 67 / 38 us).
+    if (p.rows <= 64 || columns * ((p.rows + 63) / 64) <= 256) {
         auto few = [&](auto mt) {
             constexpr int kMt = decltype(mt)::value;
             hipLaunchKernelGGL((fp8_product_few_kernel<O, kMt>),
@@ -320,6 +544,19 @@ int launch_product(const ProductArgs &p, hipStream_t st) {
         GNNAGG_HIP(hipGetLastError());
         return GNNAGG_OK;
     }
+    // Many rows against a weight that fits LDS: below about 40 000 rows bringing the weight there costs more than it saves
+    // (512 x 256 to fp32, this kernel / tiles: 20 000 rows 19 / 17 us, 65 536 rows 30 / 35 us, 1 M rows 0.40 / 0.64 ms).
+    if (p.rows >= 40000 && rows_lds(p)) {
+        if (p.blocks == 1) return launch_rows<O, 1>(p, st);
+        if (p.blocks == 2) return launch_rows<O, 2>(p, st);
+        if (p.blocks == 3) return launch_rows<O, 3>(p, st);
+        return launch_rows<O, 4>(p, st);
+    }
+    // Tiles of 256 x 256 feed the matrix units better, but a compute unit holds one block of them and nothing runs beside its
+    // start and end: they pay where the contraction is long and there are two rounds of them (to bf16, 256 / 128:
+    // 8192^3 0.67 / 0.78 ms, 8192 x 4096 x 4096 180 / 178 us, 4096^3 95 / 92 us, 100 000 x 1024 x 1024 253 / 233 us).
+    const int64_t large = ((p.rows + 255) / 256) * ((p.n + 255) / 256);
+    if (p.blocks >= 32 && large >= 512) return launch_tiles<O, 4, 4, 2, 2>(p, st);
     return launch_tiles<O, 2, 2, 2, 2>(p, st);
 }
 
@@ -339,7 +576,7 @@ extern "C" int gnnagg_fp8_product(const uint8_t *x, const uint8_t *x_scales, con
     GNNAGG_REQUIRE(out_stride >= n, "the output row stride is below the width");
     GNNAGG_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0,
                    "codes must be 16-byte aligned");
-    if (k > (int64_t(1) << 31) || n > (int64_t(1) << 34)) return fail(GNNAGG_ERR_UNSUPPORTED, "a weight of %lld x %lld", (long long)k, (long long)n);
+    if (k > (int64_t(1) << 23) || n > (int64_t(1) << 34)) return fail(GNNAGG_ERR_UNSUPPORTED, "a weight of %lld x %lld", (long long)k, (long long)n);
     ProductArgs p{x, x_scales, w, w_scales, bias, out, scale_k_stride, scale_n_stride, out_stride, rows, n,
                   (int)(pad128(k) / kBlock8), 0};
     p.vec = vec4_rows(out, out_stride, n, out_dtype);

@@ -71,13 +71,6 @@ __device__ __forceinline__ uint32_t word(bf16x2_t h) {
     return x.u;
 }
 
-// keeps an address that is the same for the whole wave in scalar registers
-template <typename T>
-__device__ __forceinline__ const T *scalar(const T *p) {
-    asm volatile("" : "+s"(p));
-    return p;
-}
-
 // What a thread brings of one operand: four neighbouring columns of eight rows, in registers as they lie in memory (no
 // conversion, so no wait, before they are written to LDS).  The rows are the same for a whole wave: scalar addresses.
 struct XRun {
