@@ -63,37 +63,54 @@ __device__ __forceinline__ f32x4 decode4(uint32_t c) {
     return f32x4{lo.x, lo.y, hi.x, hi.y};
 }
 
-// Four consecutive values of a row of `width`, the first at column c.  VEC: the row is aligned for one wide load and
-// width % 4 == 0.  Columns past the width read as zero.
-template <bool VEC>
-__device__ __forceinline__ f32x4 load4(const float *row, int64_t c, int64_t width) {
+// Four consecutive values of a row of `width`, the first at column c, as they lie in memory (load4_raw: nothing waits for
+// them before widen) or in fp32.  VEC: the row is aligned for one wide load and width % 4 == 0.  Columns past the width
+// read as zero.
+__device__ __forceinline__ f32x4 widen(const f32x4 v) { return v; }
+__device__ __forceinline__ f32x4 widen(const u16x4 u) {
+    return f32x4{bf16_value(u.x), bf16_value(u.y), bf16_value(u.z), bf16_value(u.w)};
+}
+// (I: int where the width allows; comparisons of 64 bits are what a narrow row's time goes into.)
+template <bool VEC, typename I>
+__device__ __forceinline__ f32x4 load4_raw(const float *row, I c, I width) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (VEC) {
         if (c < width) v = *reinterpret_cast<const f32x4 *>(row + c);
-    } else {
-        if (c + 0 < width) v.x = row[c + 0];
-        if (c + 1 < width) v.y = row[c + 1];
-        if (c + 2 < width) v.z = row[c + 2];
-        if (c + 3 < width) v.w = row[c + 3];
+    } else if (width > 0) {  // four loads in bounds, what they read past the width replaced: no branch between them
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = row[c + j < width ? c + j : width - 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = c + j < width ? v[j] : 0.0f;
     }
     return v;
 }
-template <bool VEC>
-__device__ __forceinline__ f32x4 load4(const bf16_t *row, int64_t c, int64_t width) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+template <bool VEC, typename I>
+__device__ __forceinline__ u16x4 load4_raw(const bf16_t *row, I c, I width) {
+    u16x4 v = {0, 0, 0, 0};
     if (VEC) {
-        if (c < width) {
-            const u16x4 u = *reinterpret_cast<const u16x4 *>(row + c);
-            v = f32x4{bf16_value(u.x), bf16_value(u.y), bf16_value(u.z), bf16_value(u.w)};
-        }
-    } else {
-        if (c + 0 < width) v.x = bf16_value(row[c + 0].bits);
-        if (c + 1 < width) v.y = bf16_value(row[c + 1].bits);
-        if (c + 2 < width) v.z = bf16_value(row[c + 2].bits);
-        if (c + 3 < width) v.w = bf16_value(row[c + 3].bits);
+        if (c < width) v = *reinterpret_cast<const u16x4 *>(row + c);
+    } else if (width > 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = row[c + j < width ? c + j : width - 1].bits;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = c + j < width ? v[j] : (unsigned short)0;
     }
     return v;
 }
+template <bool VEC, typename T, typename I>
+__device__ __forceinline__ f32x4 load4(const T *row, I c, I width) {
+    return widen(load4_raw<VEC>(row, c, width));
+}
+template <typename T>
+struct RawOf;
+template <>
+struct RawOf<float> {
+    typedef f32x4 type;
+};
+template <>
+struct RawOf<bf16_t> {
+    typedef u16x4 type;
+};
 
 // two fp32 values -> two bf16 in one word (round to nearest even, the hardware's conversion)
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
@@ -105,8 +122,8 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
     return x.u;
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store4(float *row, int64_t c, int64_t width, const f32x4 v) {
+template <bool VEC, typename I>
+__device__ __forceinline__ void store4(float *row, I c, I width, const f32x4 v) {
     if (VEC) {
         if (c < width) *reinterpret_cast<f32x4 *>(row + c) = v;
     } else {
@@ -116,8 +133,8 @@ __device__ __forceinline__ void store4(float *row, int64_t c, int64_t width, con
         if (c + 3 < width) row[c + 3] = v.w;
     }
 }
-template <bool VEC>
-__device__ __forceinline__ void store4(bf16_t *row, int64_t c, int64_t width, const f32x4 v) {
+template <bool VEC, typename I>
+__device__ __forceinline__ void store4(bf16_t *row, I c, I width, const f32x4 v) {
     const uint32_t lo = bf16_pair(v.x, v.y), hi = bf16_pair(v.z, v.w);
     if (VEC) {
         if (c < width) *reinterpret_cast<uint2 *>(row + c) = uint2{lo, hi};

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T *__restric
     for (int i = 0; i < 16; ++i) {
         const int64_t row = k0 + r0 + 8 * i;
         v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (row < k) v[i] = load4<VEC>(w + row * w_stride, n0 + 4 * cq, n);
+        if (row < k) v[i] = load4<VEC>(w + row * w_stride, (int64_t)(n0 + 4 * cq), n);
         top = fmaxf(top, finite_magnitude(v[i]));
     }
 #pragma unroll

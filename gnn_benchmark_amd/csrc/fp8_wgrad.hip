@@ -295,7 +295,7 @@ __global__ __launch_bounds__(512, 2) void fp8_wgrad_kernel(const WgradArgs p) {
         if (tid < 64) {
             f32x4 total = parts[tid];
             for (int q = 1; q < 4; ++q) total += parts[tid + 64 * q];
-            store4<false>(p.bias_out + slice * p.n, w.n0 + 4 * tid, p.n, total);
+            store4<false>(p.bias_out + slice * p.n, (int64_t)(w.n0 + 4 * tid), p.n, total);
         }
     }
 }

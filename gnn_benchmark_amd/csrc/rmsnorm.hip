@@ -23,8 +23,9 @@ struct NormArgs {
     void *h, *y;
     uint8_t *codes, *scales;
     int64_t x_stride, residual_stride, h_stride, y_stride;
-    int64_t rows, width, padded;
-    double eps;
+    int64_t rows;
+    int width, padded;
+    double inv_width, eps;
     int relu, weight_bf16;
 };
 
@@ -33,17 +34,12 @@ struct NormBackwardArgs {
     void *grad_x;
     float *partial;
     int64_t grad_y_stride, grad_h_stride, h_stride, grad_x_stride;
-    int64_t rows, width;
-    double eps;
+    int64_t rows;
+    int width;
+    double inv_width, eps;
     int relu, weight_bf16;
 };
 
-template <int W>
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int s = W / 2; s >= 1; s >>= 1) v += __shfl_xor(v, s, W);
-    return v;
-}
 template <int W>
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
@@ -51,98 +47,187 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
-// the sum over a row's TPR threads, in every one of them; `slot`: 16 doubles of LDS where the row has a whole block
-template <int TPR>
-__device__ __forceinline__ double row_sum(double v, double *slot) {
-    if constexpr (TPR <= 64) {
-        return wave_sum<TPR>(v);
-    } else {
-        v = wave_sum<64>(v);
-        if (threadIdx.x % 64 == 0) slot[threadIdx.x / 64] = v;
-        __syncthreads();
-        double s = slot[0];
+// The sums over a row's TPR threads, in every one of them, of U rows at once.  `slot`: U x 16 doubles of LDS where the row
+// has a whole block; two of them, taken in turn, so that one barrier a sum is enough.
+template <int TPR, int U>
+__device__ __forceinline__ void row_sums(double (&v)[U], double (*slot)[16]) {
 #pragma unroll
-        for (int q = 1; q < TPR / 64; ++q) s += slot[q];
-        __syncthreads();
-        return s;
+    for (int s = (TPR < 64 ? TPR : 64) / 2; s >= 1; s >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] += __shfl_xor(v[u], s, TPR < 64 ? TPR : 64);
+    if constexpr (TPR > 64) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (threadIdx.x % 64 == 0) slot[u][threadIdx.x / 64] = v[u];
+        lds_barrier();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v[u] = slot[u][0];
+#pragma unroll
+            for (int q = 1; q < TPR / 64; ++q) v[u] += slot[u][q];
+        }
     }
 }
 
-template <bool VEC>
-__device__ __forceinline__ f32x4 load_weight(const void *w, int is_bf16, int64_t c, int64_t width) {
-    return is_bf16 ? load4<VEC>(static_cast<const bf16_t *>(w), c, width) : load4<VEC>(static_cast<const float *>(w), c, width);
-}
+// Which columns run k of a row's thread l holds: four neighbours, or, SPREAD, one of each four stretches of TPR.  Rows that
+// cannot be moved in wide pieces are read and written in stretches: a store of every fourth value is a request for every
+// line (1 M x 47: 133 + 193 us forward and backward, 78 + 135 in stretches).
+template <int TPR, bool VEC, bool SPREAD>
+struct Columns {
+    template <typename T>
+    static __device__ __forceinline__ typename RawOf<T>::type load(const T *row, int l, int k, int width) {
+        if constexpr (!SPREAD) {
+            return load4_raw<VEC>(row, 4 * (l + k * TPR), width);
+        } else {
+            typename RawOf<T>::type v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = (4 * k + j) * TPR + l;
+                const T x = row[c < width ? c : width - 1];
+                if constexpr (sizeof(T) == 4) v[j] = c < width ? x : 0.0f;
+                else v[j] = c < width ? x.bits : (unsigned short)0;
+            }
+            return v;
+        }
+    }
+    template <typename T>
+    static __device__ __forceinline__ void store(T *row, int l, int k, int width, const f32x4 v) {
+        if constexpr (!SPREAD) {
+            store4<VEC>(row, 4 * (l + k * TPR), width, v);
+        } else {
+            const f32x4 r = rounded(row, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = (4 * k + j) * TPR + l;
+                if (c < width) {
+                    if constexpr (sizeof(T) == 4) row[c] = r[j];
+                    else row[c].bits = (unsigned short)(__float_as_uint(r[j]) >> 16);
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ f32x4 weight(const void *w, int is_bf16, int l, int k, int width) {
+        return is_bf16 ? widen(load(static_cast<const bf16_t *>(w), l, k, width))
+                       : widen(load(static_cast<const float *>(w), l, k, width));
+    }
+};
 
-// h and the sum of its squares; returns r
-template <int TPR, int NV>
-__device__ __forceinline__ float inverse_rms(const f32x4 (&h)[NV], int64_t width, double eps, double *slot) {
-    double q = 0.0;
+// r of U rows
+template <int TPR, int U, int NV>
+__device__ __forceinline__ void inverse_rms(const f32x4 (&h)[U][NV], double inv_width, double eps, double (*slot)[16],
+                                            float (&r)[U]) {
+    double q[U];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int u = 0; u < U; ++u) {
+        q[u] = 0.0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q = __builtin_fma((double)h[k][j], (double)h[k][j], q);
-    q = row_sum<TPR>(q, slot);
-    return (float)(1.0 / __builtin_sqrt(q / (double)width + eps));
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[u] = __builtin_fma((double)h[u][k][j], (double)h[u][k][j], q[u]);
+    }
+    row_sums<TPR, U>(q, slot);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        // 1 / sqrt: the hardware's estimate (2^-26) and a Newton step, beyond fp32 by far.  The library's square root and
+        // division in 64 bits are some 60 instructions (8192 x 5120 bf16, forward: 103 us with them, 88 without).
+        const double a = q[u] * inv_width + eps, y = __builtin_amdgcn_rsq(a);
+        r[u] = (float)(y * __builtin_fma(-0.5 * a * y, y, 1.5));
+    }
 }
 
 constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
+// Rows a thread works on at once: narrow rows are a few hundred bytes a wave, too little on the way to hide the way.
+constexpr int rows_at_once(int tpr, int nv) { return tpr > 64 ? 1 : nv == 1 ? 4 : nv == 2 ? 2 : 1; }
 
 template <typename T, int TPR, int NV, bool VEC, bool FP8>
 __global__ __launch_bounds__(block_of(TPR)) void rms_norm_kernel(const NormArgs p) {
-    constexpr int kGroups = block_of(TPR) / TPR;
-    __shared__ double slot[16];
+    constexpr int kGroups = block_of(TPR) / TPR, U = rows_at_once(TPR, NV);
+    constexpr bool kAhead = TPR == 256 || (TPR == 1024 && NV <= 2);  // a block's next row is asked for before its barrier
+    typedef typename RawOf<T>::type Raw;
+    typedef Columns<TPR, VEC, !VEC && !FP8> C;
+    __shared__ double slots[2][1][16];
     const int l = (int)threadIdx.x % TPR;
     f32x4 w[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) w[k] = load_weight<VEC>(p.weight, p.weight_bf16, 4 * (l + k * TPR), p.width);
-    // the threads of a row stay or leave together: shuffles and barriers never miss one
-    for (int64_t row = (int64_t)blockIdx.x * kGroups + (int)threadIdx.x / TPR; row < p.rows;
-         row += (int64_t)gridDim.x * kGroups) {
-        const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
-        f32x4 h[NV];
+    for (int k = 0; k < NV; ++k) w[k] = C::weight(p.weight, p.weight_bf16, l, k, p.width);
+    Raw x[U][NV], res[U][NV];
+    auto load = [&](int64_t row) {  // rows row, row + kGroups, ...; those past the end read the last one
 #pragma unroll
-        for (int k = 0; k < NV; ++k) h[k] = load4<VEC>(x, 4 * (l + k * TPR), p.width);
-        if (p.residual) {
-            const T *res = static_cast<const T *>(p.residual) + row * p.residual_stride;
-            T *ho = static_cast<T *>(p.h) + row * p.h_stride;
+        for (int u = 0; u < U; ++u) {
+            const int64_t m = row + u * kGroups < p.rows ? row + u * kGroups : p.rows - 1;
+            const T *xr = static_cast<const T *>(p.x) + m * p.x_stride;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) h[k] = rounded(x, h[k] + load4<VEC>(res, 4 * (l + k * TPR), p.width));
+            for (int k = 0; k < NV; ++k) x[u][k] = C::load(xr, l, k, p.width);
+            if (p.residual) {
+                const T *rr = static_cast<const T *>(p.residual) + m * p.residual_stride;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) store4<VEC>(ho, 4 * (l + k * TPR), p.width, h[k]);
-        }
-        const float r = inverse_rms<TPR, NV>(h, p.width, p.eps, slot);
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            h[k] = h[k] * r * w[k];
-            if (p.relu) {  // (a NaN stays one)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) h[k][j] = h[k][j] < 0.0f ? 0.0f : h[k][j];
+                for (int k = 0; k < NV; ++k) res[u][k] = C::load(rr, l, k, p.width);
             }
         }
-        if constexpr (!FP8) {
-            T *y = static_cast<T *>(p.y) + row * p.y_stride;
+    };
+    const int64_t stride = (int64_t)gridDim.x * kGroups * U;
+    int64_t first = (int64_t)blockIdx.x * kGroups * U + (int)threadIdx.x / TPR;
+    int parity = 0;
+    if (kAhead) load(first);
+    // the threads of a row stay or leave together (a whole block's where there is a barrier)
+    for (; first < p.rows; first += stride, parity ^= 1) {
+        if (!kAhead) load(first);
+        f32x4 h[U][NV];
 #pragma unroll
-            for (int k = 0; k < NV; ++k) store4<VEC>(y, 4 * (l + k * TPR), p.width, h[k]);
-        } else {
-            // Run k of the row's threads covers 4 * TPR columns: either whole blocks of 128, 32 neighbouring threads
-            // each, or a part of one that the next runs complete.
-            constexpr int kThreads = TPR < 32 ? TPR : 32;    // threads that share a block
-            constexpr int kRuns = TPR < 32 ? 32 / TPR : 1;   // runs that share a block
-            uint8_t *codes = p.codes + row * p.padded;
-            uint8_t *scales = p.scales + row * (p.padded / kBlock8);
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int k0 = 0; k0 < NV; k0 += kRuns) {
-                float top = 0.0f;
+            for (int k = 0; k < NV; ++k) h[u][k] = widen(x[u][k]);
+            if (p.residual) {
 #pragma unroll
-                for (int k = k0; k < k0 + kRuns && k < NV; ++k) top = fmaxf(top, finite_magnitude(h[k]));
-                const int e = block_exponent(wave_max<kThreads>(top));
-                const float inv = pow2(-e);
+                for (int k = 0; k < NV; ++k) h[u][k] = rounded(static_cast<const T *>(p.x), h[u][k] + widen(res[u][k]));
+                const int64_t row = first + u * kGroups;
+                if (U == 1 || row < p.rows) {
+                    T *ho = static_cast<T *>(p.h) + row * p.h_stride;
 #pragma unroll
-                for (int k = k0; k < k0 + kRuns; ++k) {      // (runs past NV hold a narrow row's padding)
-                    const int64_t c = 4 * (l + k * TPR);
-                    if (c >= p.padded) continue;
-                    *reinterpret_cast<uint32_t *>(codes + c) = k < NV ? encode4(h[k < NV ? k : 0], inv) : 0u;
-                    if (c % kBlock8 == 0) scales[c / kBlock8] = (uint8_t)(e + 127);
+                    for (int k = 0; k < NV; ++k) C::store(ho, l, k, p.width, h[u][k]);
+                }
+            }
+        }
+        if (kAhead && first + stride < p.rows) load(first + stride);
+        float r[U];
+        inverse_rms<TPR, U, NV>(h, p.inv_width, p.eps, slots[parity], r);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t row = first + u * kGroups;
+            if (U > 1 && row >= p.rows) continue;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                h[u][k] = h[u][k] * r[u] * w[k];
+                if (p.relu) {  // (a NaN stays one)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) h[u][k][j] = h[u][k][j] < 0.0f ? 0.0f : h[u][k][j];
+                }
+            }
+            if constexpr (!FP8) {
+                T *y = static_cast<T *>(p.y) + row * p.y_stride;
+#pragma unroll
+                for (int k = 0; k < NV; ++k) C::store(y, l, k, p.width, h[u][k]);
+            } else {
+                // Run k of the row's threads covers 4 * TPR columns: either whole blocks of 128, 32 neighbouring threads
+                // each, or a part of one that the next runs complete.
+                constexpr int kThreads = TPR < 32 ? TPR : 32;    // threads that share a block
+                constexpr int kRuns = TPR < 32 ? 32 / TPR : 1;   // runs that share a block
+                uint8_t *codes = p.codes + row * p.padded;
+                uint8_t *scales = p.scales + row * (p.padded / kBlock8);
+#pragma unroll
+                for (int k0 = 0; k0 < NV; k0 += kRuns) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int k = k0; k < k0 + kRuns && k < NV; ++k) top = fmaxf(top, finite_magnitude(h[u][k]));
+                    const int e = block_exponent(wave_max<kThreads>(top));
+                    const float inv = pow2(-e);
+#pragma unroll
+                    for (int k = k0; k < k0 + kRuns; ++k) {      // (runs past NV hold a narrow row's padding)
+                        const int c = 4 * (l + k * TPR);
+                        if (c >= p.padded) continue;
+                        *reinterpret_cast<uint32_t *>(codes + c) = k < NV ? encode4(h[u][k < NV ? k : 0], inv) : 0u;
+                        if (c % kBlock8 == 0) scales[c / kBlock8] = (uint8_t)(e + 127);
+                    }
                 }
             }
         }
@@ -151,50 +236,92 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_kernel(const NormArgs 
 
 template <typename T, int TPR, int NV, bool VEC>
 __global__ __launch_bounds__(block_of(TPR)) void rms_norm_backward_kernel(const NormBackwardArgs p) {
-    constexpr int kGroups = block_of(TPR) / TPR;
-    __shared__ double slot[16];
+    constexpr int kGroups = block_of(TPR) / TPR, U = rows_at_once(TPR, NV);
+    constexpr bool kAhead = TPR == 256;
+    constexpr bool kLean = TPR == 1024;  // 128 registers a thread: the weight and grad_h are read where they are used
+    typedef typename RawOf<T>::type Raw;
+    typedef Columns<TPR, VEC, !VEC> C;
+    __shared__ double slots[2][2][1][16];
     __shared__ f32x4 sums[kGroups > 1 ? 256 : 1];
     const int l = (int)threadIdx.x % TPR;
-    f32x4 w[NV], gw_sum[NV];
+    f32x4 w_kept[kLean ? 1 : NV], gw_sum[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        w[k] = load_weight<VEC>(p.weight, p.weight_bf16, 4 * (l + k * TPR), p.width);
+        if (!kLean) w_kept[kLean ? 0 : k] = C::weight(p.weight, p.weight_bf16, l, k, p.width);
         gw_sum[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int64_t row = (int64_t)blockIdx.x * kGroups + (int)threadIdx.x / TPR; row < p.rows;
-         row += (int64_t)gridDim.x * kGroups) {
-        const T *hr = static_cast<const T *>(p.h) + row * p.h_stride;
-        f32x4 h[NV], g[NV];
+    auto weight = [&](int k) { return kLean ? C::weight(p.weight, p.weight_bf16, l, k, p.width) : w_kept[kLean ? 0 : k]; };
+    Raw hx[U][NV], gx[U][NV], gh[U][NV];
+    auto load = [&](int64_t row) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) h[k] = load4<VEC>(hr, 4 * (l + k * TPR), p.width);
-        const T *gr = static_cast<const T *>(p.grad_y) + row * p.grad_y_stride;
+        for (int u = 0; u < U; ++u) {
+            const int64_t m = row + u * kGroups < p.rows ? row + u * kGroups : p.rows - 1;
+            const T *hr = static_cast<const T *>(p.h) + m * p.h_stride;
+            const T *gr = static_cast<const T *>(p.grad_y) + m * p.grad_y_stride;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) g[k] = load4<VEC>(gr, 4 * (l + k * TPR), p.width);
-        const float r = inverse_rms<TPR, NV>(h, p.width, p.eps, slot);
-        double s = 0.0;
+            for (int k = 0; k < NV; ++k) hx[u][k] = C::load(hr, l, k, p.width);
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const f32x4 z = h[k] * r;
-            if (p.relu) {  // exactly the values that the forward cut or found at zero
-                const f32x4 y = z * w[k];
+            for (int k = 0; k < NV; ++k) gx[u][k] = C::load(gr, l, k, p.width);
+            if (!kLean && p.grad_h) {
+                const T *sr = static_cast<const T *>(p.grad_h) + m * p.grad_h_stride;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) g[k][j] = y[j] > 0.0f ? g[k][j] : 0.0f;
+                for (int k = 0; k < NV; ++k) gh[u][k] = C::load(sr, l, k, p.width);
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) gw_sum[k][j] = __builtin_fmaf(g[k][j], z[j], gw_sum[k][j]);
-            g[k] = g[k] * w[k];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s = __builtin_fma((double)g[k][j], (double)h[k][j], s);
         }
-        s = row_sum<TPR>(s, slot);
-        const float t = (float)(s * (double)r / (double)p.width);  // (r^3 alone would leave fp32's range for large rows)
-        const T *gh = p.grad_h ? static_cast<const T *>(p.grad_h) + row * p.grad_h_stride : nullptr;
-        T *out = static_cast<T *>(p.grad_x) + row * p.grad_x_stride;
+    };
+    const int64_t stride = (int64_t)gridDim.x * kGroups * U;
+    int64_t first = (int64_t)blockIdx.x * kGroups * U + (int)threadIdx.x / TPR;
+    int parity = 0;
+    if (kAhead) load(first);
+    for (; first < p.rows; first += stride, parity ^= 1) {
+        if (!kAhead) load(first);
+        f32x4 h[U][NV], g[U][NV], more[U][NV];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            f32x4 d = (g[k] - h[k] * r * t) * r;
-            if (gh) d += load4<VEC>(gh, 4 * (l + k * TPR), p.width);
-            store4<VEC>(out, 4 * (l + k * TPR), p.width, d);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                h[u][k] = widen(hx[u][k]);
+                g[u][k] = widen(gx[u][k]);
+                if (!kLean) more[u][k] = p.grad_h ? widen(gh[u][k]) : f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        if (kAhead && first + stride < p.rows) load(first + stride);
+        float r[U];
+        inverse_rms<TPR, U, NV>(h, p.inv_width, p.eps, slots[parity][0], r);
+        double s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s[u] = 0.0;
+            const bool in = U == 1 || first + u * kGroups < p.rows;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const f32x4 z = h[u][k] * r[u], w = weight(k);
+                if (p.relu) {  // exactly the values that the forward cut or found at zero
+                    const f32x4 y = z * w;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) g[u][k][j] = y[j] > 0.0f ? g[u][k][j] : 0.0f;
+                }
+                if (in) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) gw_sum[k][j] = __builtin_fmaf(g[u][k][j], z[j], gw_sum[k][j]);
+                }
+                g[u][k] = g[u][k] * w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[u] = __builtin_fma((double)g[u][k][j], (double)h[u][k][j], s[u]);
+            }
+        }
+        row_sums<TPR, U>(s, slots[parity][1]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t row = first + u * kGroups;
+            if (U > 1 && row >= p.rows) continue;
+            const float t = (float)(s[u] * (double)r[u] * p.inv_width);  // (r^3 would leave fp32's range for large rows)
+            T *out = static_cast<T *>(p.grad_x) + row * p.grad_x_stride;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                f32x4 d = (g[u][k] - h[u][k] * r[u] * t) * r[u];
+                if (p.grad_h) d += kLean ? widen(C::load(static_cast<const T *>(p.grad_h) + row * p.grad_h_stride, l, k, p.width)) : more[u][k];
+                C::store(out, l, k, p.width, d);
+            }
         }
     }
     // the block's rows' share of the weight gradient: its groups' sums in group order
@@ -209,7 +336,7 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_backward_kernel(const 
             if (threadIdx.x < TPR)
                 for (int q = 1; q < kGroups; ++q) total += sums[l + q * TPR];
         }
-        if (threadIdx.x < TPR) store4<false>(partial, 4 * (l + k * TPR), p.width, total);
+        if (threadIdx.x < TPR) Columns<TPR, false, !VEC>::store(partial, l, k, p.width, total);
     }
 }
 
@@ -274,8 +401,8 @@ void for_norm_shape(const NormShape s, F &&launch) {
 
 int64_t backward_blocks(int64_t rows, int64_t width) {
     const int tpr = norm_shape(width).tpr;
-    const int64_t groups = block_of(tpr) / tpr;
-    const int64_t need = (rows + groups - 1) / groups;
+    const int64_t at_once = block_of(tpr) / tpr * rows_at_once(tpr, norm_shape(width).nv);
+    const int64_t need = (rows + at_once - 1) / at_once;
     return need < 1024 ? need : 1024;  // four blocks a CU; 1024 partial rows are added in about 5 us
 }
 
@@ -294,9 +421,11 @@ int run_norm(const NormArgs &p, int dtype, int weight_dtype, bool fp8, hipStream
                      vec4_rows(p.h, p.h_stride, p.width, dtype) && vec4_rows(p.y, p.y_stride, p.width, dtype) &&
                      vec4_rows(p.weight, 4, p.width, weight_dtype);
     for_norm_shape(norm_shape(p.width), [&](auto tpr, auto nv) {
-        constexpr int kTpr = decltype(tpr)::value, kNv = decltype(nv)::value, kGroups = block_of(kTpr) / kTpr;
-        const int64_t need = (p.rows + kGroups - 1) / kGroups;
-        const dim3 grid((unsigned)(need < 256 * 32 ? need : 256 * 32));
+        constexpr int kTpr = decltype(tpr)::value, kNv = decltype(nv)::value;
+        constexpr int kAtOnce = block_of(kTpr) / kTpr * rows_at_once(kTpr, kNv);
+        const int64_t need = (p.rows + kAtOnce - 1) / kAtOnce;
+        const int64_t most = kTpr > 64 ? 256 * 4 : 256 * 32;  // blocks that keep a row ahead stay for several rows
+        const dim3 grid((unsigned)(need < most ? need : most));
         auto go = [&](auto type, auto v, auto q) {
             hipLaunchKernelGGL((rms_norm_kernel<decltype(type), kTpr, kNv, decltype(v)::value, decltype(q)::value>), grid,
                                dim3(block_of(kTpr)), 0, st, p);
@@ -344,7 +473,7 @@ static int norm_forward(const void *x, int64_t x_stride, const void *residual, i
                        (fp8 || y_stride >= width), "a row stride is below the width");
     GNNAGG_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 4 == 0, "codes must be 4-byte aligned");
     NormArgs p{x, residual, weight, h, y, codes, scales, x_stride, residual_stride, h_stride, y_stride,
-               rows, width, pad128(width), eps, relu, weight_dtype == GNNAGG_BF16};
+               rows, (int)width, (int)pad128(width), 1.0 / (double)width, eps, relu, weight_dtype == GNNAGG_BF16};
     return run_norm(p, dtype, weight_dtype, fp8, static_cast<hipStream_t>(stream));
 }
 
@@ -384,7 +513,7 @@ extern "C" int gnnagg_rms_norm_backward(const void *grad_y, int64_t grad_y_strid
                        reinterpret_cast<uintptr_t>(workspace) % 4 == 0,
                    "workspace of %lld bytes is too small or misaligned", (long long)workspace_bytes);
     NormBackwardArgs p{grad_y, grad_h, h, weight, grad_x, static_cast<float *>(workspace), grad_y_stride, grad_h_stride,
-                       h_stride, grad_x_stride, rows, width, eps, relu, weight_dtype == GNNAGG_BF16};
+                       h_stride, grad_x_stride, rows, (int)width, 1.0 / (double)width, eps, relu, weight_dtype == GNNAGG_BF16};
     const bool vec = vec4_rows(grad_y, grad_y_stride, width, dtype) && vec4_rows(grad_h, grad_h_stride, width, dtype) &&
                      vec4_rows(h, h_stride, width, dtype) && vec4_rows(grad_x, grad_x_stride, width, dtype) &&
                      vec4_rows(weight, 4, width, weight_dtype);

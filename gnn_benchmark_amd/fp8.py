@@ -32,10 +32,15 @@ def dtype_code(dtype: torch.dtype, what: str) -> int:
 
 
 def check_gpu(t: torch.Tensor, what: str, device=None) -> None:
+    if t.is_cuda and (device is None or t.device == device):
+        return
     if not t.is_cuda:
         raise RuntimeError(f"Input mismatch: {what} must be a GPU (HIP) tensor")
-    if device is not None and t.device != device:
-        raise RuntimeError(f"Input mismatch: {what} is on {t.device}, the other operands on {device}")
+    raise RuntimeError(f"Input mismatch: {what} is on {t.device}, the other operands on {device}")
+
+
+def address(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def as_rows(t: torch.Tensor) -> torch.Tensor:
@@ -106,9 +111,9 @@ def _quantize_rows(x: torch.Tensor) -> QuantizedRows:
         raise RuntimeError("Input mismatch: x must be [rows, width] with a width above zero")
     x = as_rows(x)
     q = QuantizedRows.empty(x.size(0), x.size(1), x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().gnnagg_fp8_quantize_rows(_lib.ptr(x), row_stride(x), _lib.ptr(q.codes), _lib.ptr(q.scales),
-                                                       x.size(0), x.size(1), code, _lib.current_stream(x.device)))
+    with _lib.on_device(x.device):
+        _lib.check(_lib.lib().gnnagg_fp8_quantize_rows(address(x), row_stride(x), address(q.codes), address(q.scales),
+                                                       x.size(0), x.size(1), code, _lib.raw_stream(x.device)))
     return q
 
 
@@ -133,9 +138,9 @@ def _quantize_weight(w: torch.Tensor, by_output: bool, by_input: bool) -> Quanti
     codes = torch.empty(n, padded(k), dtype=torch.float8_e4m3fn, device=dev) if by_output else None
     codes_by_input = torch.empty(k, padded(n), dtype=torch.float8_e4m3fn, device=dev) if by_input else None
     scales = torch.empty(padded(k) // BLOCK, padded(n) // BLOCK, dtype=torch.float8_e8m0fnu, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().gnnagg_fp8_quantize_weight(_lib.ptr(w), row_stride(w), _lib.ptr(codes), _lib.ptr(codes_by_input),
-                                                         _lib.ptr(scales), k, n, code, _lib.current_stream(dev)))
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().gnnagg_fp8_quantize_weight(address(w), row_stride(w), address(codes), address(codes_by_input),
+                                                         address(scales), k, n, code, _lib.raw_stream(dev)))
     return QuantizedWeight(k, n, codes, scales, codes_by_input)
 
 
@@ -185,10 +190,10 @@ def _product(x, weight, bias, out_dtype, out=None, input_gradient=False):
         if tuple(out.shape) != (rows, wide) or as_rows(out) is not out:
             raise RuntimeError("Input mismatch: out must be [rows, outputs] with contiguous rows")
     stride_k, stride_n = scales.stride()[::-1] if input_gradient else scales.stride()
-    with torch.cuda.device(device):
+    with _lib.on_device(device):
         _lib.check(_lib.lib().gnnagg_fp8_product(
-            _lib.ptr(x.codes), _lib.ptr(x.scales), _lib.ptr(codes), _lib.ptr(scales), stride_k, stride_n, _lib.ptr(bias),
-            _lib.ptr(out), row_stride(out), code, rows, inner, wide, _lib.current_stream(device)))
+            address(x.codes), address(x.scales), address(codes), address(scales), stride_k, stride_n, address(bias),
+            address(out), row_stride(out), code, rows, inner, wide, _lib.raw_stream(device)))
     return out
 
 
@@ -206,10 +211,10 @@ def weight_gradient(x: QuantizedRows, g: torch.Tensor, with_bias: bool = False):
     grad_w = torch.empty(k, n, dtype=torch.float32, device=device)
     grad_b = torch.empty(n, dtype=torch.float32, device=device) if with_bias else None
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    with torch.cuda.device(device):
+    with _lib.on_device(device):
         _lib.check(L.gnnagg_fp8_weight_gradient(
-            _lib.ptr(x.codes), _lib.ptr(x.scales), _lib.ptr(g), row_stride(g), code, _lib.ptr(grad_w), _lib.ptr(grad_b),
-            _lib.ptr(workspace), nbytes, rows, k, n, _lib.current_stream(device)))
+            address(x.codes), address(x.scales), address(g), row_stride(g), code, address(grad_w), address(grad_b),
+            address(workspace), nbytes, rows, k, n, _lib.raw_stream(device)))
     return (grad_w, grad_b) if with_bias else grad_w
 
 

@@ -8,7 +8,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .fp8 import QuantizedRows, _refuse_grad, as_rows, check_gpu, dtype_code, row_stride
+from .fp8 import QuantizedRows, _refuse_grad, address, as_rows, check_gpu, dtype_code, row_stride
 
 
 def check_norm(x, weight, residual) -> None:
@@ -37,24 +37,24 @@ def _forward(x, weight, eps, residual, relu, y=None):
     rows, res, w, h = _operands(x, weight, residual)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if y is None else y
     yr = y.view(-1, x.size(-1)) if y.dim() != 2 else y
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x.device):
         _lib.check(_lib.lib().gnnagg_rms_norm(
-            _lib.ptr(rows), row_stride(rows), _lib.ptr(res), 0 if res is None else row_stride(res), _lib.ptr(w),
-            dtype_code(w.dtype, "the norm's weight"), float(eps), 1 if relu else 0, _lib.ptr(h),
-            0 if h is None else x.size(-1), _lib.ptr(yr), row_stride(yr), rows.size(0), rows.size(1),
-            dtype_code(x.dtype, "x"), _lib.current_stream(x.device)))
+            address(rows), row_stride(rows), address(res), 0 if res is None else row_stride(res), address(w),
+            dtype_code(w.dtype, "the norm's weight"), float(eps), 1 if relu else 0, address(h),
+            0 if h is None else x.size(-1), address(yr), row_stride(yr), rows.size(0), rows.size(1),
+            dtype_code(x.dtype, "x"), _lib.raw_stream(x.device)))
     return y, h
 
 
 def _forward_fp8(x, weight, eps, residual, relu):
     rows, res, w, h = _operands(x, weight, residual)
     q = QuantizedRows.empty(rows.size(0), rows.size(1), x.device)
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x.device):
         _lib.check(_lib.lib().gnnagg_rms_norm_fp8(
-            _lib.ptr(rows), row_stride(rows), _lib.ptr(res), 0 if res is None else row_stride(res), _lib.ptr(w),
-            dtype_code(w.dtype, "the norm's weight"), float(eps), 1 if relu else 0, _lib.ptr(h),
-            0 if h is None else x.size(-1), _lib.ptr(q.codes), _lib.ptr(q.scales), rows.size(0), rows.size(1),
-            dtype_code(x.dtype, "x"), _lib.current_stream(x.device)))
+            address(rows), row_stride(rows), address(res), 0 if res is None else row_stride(res), address(w),
+            dtype_code(w.dtype, "the norm's weight"), float(eps), 1 if relu else 0, address(h),
+            0 if h is None else x.size(-1), address(q.codes), address(q.scales), rows.size(0), rows.size(1),
+            dtype_code(x.dtype, "x"), _lib.raw_stream(x.device)))
     return q, (x if h is None else h)
 
 
@@ -70,12 +70,12 @@ def _backward(grad_y, grad_h, h, weight, eps, relu):
     grad_x = torch.empty(shape, dtype=h.dtype, device=h.device)
     grad_w = torch.empty(width, dtype=torch.float32, device=h.device)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
-    with torch.cuda.device(h.device):
+    with _lib.on_device(h.device):
         _lib.check(L.gnnagg_rms_norm_backward(
-            _lib.ptr(gy), row_stride(gy), _lib.ptr(gh), 0 if gh is None else row_stride(gh), _lib.ptr(h), row_stride(h),
-            _lib.ptr(w), dtype_code(w.dtype, "the norm's weight"), float(eps), 1 if relu else 0, _lib.ptr(grad_x), width,
-            _lib.ptr(grad_w), _lib.ptr(workspace), nbytes, rows, width, dtype_code(h.dtype, "x"),
-            _lib.current_stream(h.device)))
+            address(gy), row_stride(gy), address(gh), 0 if gh is None else row_stride(gh), address(h), row_stride(h),
+            address(w), dtype_code(w.dtype, "the norm's weight"), float(eps), 1 if relu else 0, address(grad_x), width,
+            address(grad_w), address(workspace), nbytes, rows, width, dtype_code(h.dtype, "x"),
+            _lib.raw_stream(h.device)))
     return grad_x, grad_w.to(weight.dtype)
 
 

@@ -16,23 +16,28 @@ from typing import List, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from .fp8 import BLOCK, dtype_code
+from .fp8 import BLOCK, address, dtype_code
 
 _FIELDS = 8  # words of a gnnagg_adamw_tensor
 
 
 def _same(tensors: Sequence[torch.Tensor], dtypes, device, what: str, count: int) -> torch.dtype:
+    """The one type of ``count`` contiguous tensors on the device.  (Mapped over the list: a Python loop over hundreds of
+    tensors takes longer than their update.)"""
     if len(tensors) != count:
         raise RuntimeError(f"Input mismatch: {len(tensors)} {what} for {count} parameters")
     kinds = {t.dtype for t in tensors}
     if len(kinds) != 1 or not kinds <= dtypes:
         raise RuntimeError(f"Input mismatch: {what} must all have one type, of " + ", ".join(sorted(map(str, dtypes))))
-    for t in tensors:
-        if t.device != device:
-            raise RuntimeError(f"Input mismatch: {what} must be on the parameters' GPU (HIP) device, one is on {t.device}")
-        if not t.is_contiguous():
-            raise RuntimeError(f"Input mismatch: {what} must be contiguous")
-    return next(iter(kinds))
+    if set(map(torch.Tensor.get_device, tensors)) != {device.index}:
+        raise RuntimeError(f"Input mismatch: {what} must be on the parameters' GPU (HIP) device")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise RuntimeError(f"Input mismatch: {what} must be contiguous")
+    return kinds.pop()
+
+
+def _sizes(tensors) -> list:
+    return list(map(torch.Tensor.numel, tensors))
 
 
 _FLOATS = {torch.float32, torch.bfloat16}
@@ -63,9 +68,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         state_dtype = _same(exp_avgs, {torch.float32, torch.float8_e4m3fn}, device, "states", count)
         _same(exp_avg_sqs, {state_dtype}, device, "states", count)
         lists = [params, grads, exp_avgs, exp_avg_sqs]
-        sizes = [p.numel() for p in params]
+        sizes = _sizes(params)
         for tensors, what in ((grads, "gradient"), (exp_avgs, "state"), (exp_avg_sqs, "state")):
-            if [t.numel() for t in tensors] != sizes:
+            if _sizes(tensors) != sizes:
                 raise RuntimeError(f"Input mismatch: a {what} has another size than its parameter")
         eight = state_dtype == torch.float8_e4m3fn
         if eight:
@@ -74,7 +79,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
             blocks = [-(-n // BLOCK) for n in sizes]
             for scales in (exp_avg_scales, exp_avg_sq_scales):
                 _same(scales, {torch.float8_e8m0fnu}, device, "scales", count)
-                if [t.numel() for t in scales] != blocks:
+                if _sizes(scales) != blocks:
                     raise RuntimeError("Input mismatch: scales hold one value for each 128 elements of their state")
             lists += [exp_avg_scales, exp_avg_sq_scales]
         elif exp_avg_scales is not None or exp_avg_sq_scales is not None:
@@ -83,7 +88,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
             if masters is None:
                 raise RuntimeError("Input mismatch: bfloat16 parameters need their float32 masters")
             _same(masters, {torch.float32}, device, "masters", count)
-            if [t.numel() for t in masters] != sizes:
+            if _sizes(masters) != sizes:
                 raise RuntimeError("Input mismatch: a master has another size than its parameter")
         elif masters is not None:
             raise RuntimeError("Input mismatch: float32 parameters have no masters")
@@ -100,16 +105,16 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                 lr = float(lr)
         records = (ctypes.c_uint64 * (_FIELDS * count))()
         for at, tensors in enumerate(lists):
-            records[at::_FIELDS] = [t.data_ptr() for t in tensors]
+            records[at::_FIELDS] = list(map(torch.Tensor.data_ptr, tensors))
         if masters is not None:
-            records[6::_FIELDS] = [t.data_ptr() for t in masters]
+            records[6::_FIELDS] = list(map(torch.Tensor.data_ptr, masters))
         records[7::_FIELDS] = sizes
-        with torch.cuda.device(device):
+        with _lib.on_device(device):
             _lib.check(_lib.lib().gnnagg_adamw_step(
-                ctypes.cast(records, ctypes.POINTER(_lib.AdamwTensor)), count, _lib.ptr(steps),
+                ctypes.cast(records, ctypes.POINTER(_lib.AdamwTensor)), count, address(steps),
                 dtype_code(param_dtype, "parameters"), dtype_code(grad_dtype, "gradients"), 8 if eight else 32, float(lr),
-                _lib.ptr(lr_tensor), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
-                int(seed) & 0xFFFFFFFF, int(first), _lib.current_stream(device)))
+                address(lr_tensor), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
+                int(seed) & 0xFFFFFFFF, int(first), _lib.raw_stream(device)))
 
 
 class AdamW(torch.optim.Optimizer):
