@@ -225,15 +225,11 @@ def _product_gradients(rows: QuantizedRows, weight: QuantizedWeight, g: torch.Te
     g = as_rows(g)
     if want_x:
         grad_x = _product(_quantize_rows(g), weight, None, x_dtype, input_gradient=True)
-    if want_w:
-        if want_b:
-            grad_w, grad_b = weight_gradient(rows, g, True)
-        else:
-            grad_w = weight_gradient(rows, g)
-        grad_w = grad_w.to(w_dtype)
-        grad_b = None if grad_b is None else grad_b.to(b_dtype)
-    elif want_b:
-        grad_b = g.float().sum(0).to(b_dtype)
+    if want_b:  # (beside a frozen weight too: the sums come with the weight gradient's pass)
+        grad_w, grad_b = weight_gradient(rows, g, True)
+        grad_w, grad_b = grad_w.to(w_dtype) if want_w else None, grad_b.to(b_dtype)
+    elif want_w:
+        grad_w = weight_gradient(rows, g).to(w_dtype)
     return grad_x, grad_w, grad_b
 
 

@@ -118,3 +118,20 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     check_norm(x, weight, residual)
     _refuse_grad(x, weight, residual)
     return _forward_fp8(x, weight, eps, residual, relu)
+
+
+class RmsNorm(torch.nn.Module):
+    """``rms_norm`` with its weight as a parameter: ``(y, h)`` of x and the residual stream so far."""
+
+    def __init__(self, width: int, eps: float = 1e-6):
+        super().__init__()
+        self.eps = eps
+        self.weight = torch.nn.Parameter(torch.ones(width))
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            self.weight.fill_(1.0)
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                relu: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+        return rms_norm(x, self.weight, self.eps, residual, relu)

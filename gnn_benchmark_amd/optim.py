@@ -54,7 +54,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     Parameters: all fp32, or all bf16 with fp32 ``masters`` (the values that are updated; the parameters receive them
     rounded).  Gradients: all fp32 or all bf16.  States: fp32 ``exp_avgs`` / ``exp_avg_sqs``, or float8_e4m3fn codes of m
     and sqrt(v) with ``exp_avg_scales`` / ``exp_avg_sq_scales`` (float8_e8m0fnu, one for each 128 elements).  ``lr``: a
-    number, or an fp32 scalar on the device that is read when the step runs.  ``first``: number of the first tensor for
+    number, or an fp32 scalar on the device that is read when the step runs.  No tensor that is written may overlap another
+(the same one twice is refused).  ``first``: number of the first tensor for
     the 8-bit states' random bits, where a list is split over calls."""
     count = len(params)
     if count == 0:
@@ -104,10 +105,15 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
             else:
                 lr = float(lr)
         records = (ctypes.c_uint64 * (_FIELDS * count))()
-        for at, tensors in enumerate(lists):
-            records[at::_FIELDS] = list(map(torch.Tensor.data_ptr, tensors))
-        if masters is not None:
-            records[6::_FIELDS] = list(map(torch.Tensor.data_ptr, masters))
+        written = []
+        for at, tensors in enumerate(lists + ([] if masters is None else [masters])):
+            addresses = list(map(torch.Tensor.data_ptr, tensors))
+            records[at if tensors is not masters else 6::_FIELDS] = addresses
+            if tensors is not grads:
+                written += addresses
+        written = [a for a in written if a]  # (an empty tensor has none)
+        if len(set(written)) != len(written):
+            raise RuntimeError("Input mismatch: the same memory twice among parameters, states and masters")
         records[7::_FIELDS] = sizes
         with _lib.on_device(device):
             _lib.check(_lib.lib().gnnagg_adamw_step(

@@ -20,14 +20,24 @@ the left half (the reference's ``out /= graph.in_degrees``) or, for a graph prep
 
 Dropout takes explicit keep masks (seeded, reproducible); without them a mask is drawn with
 ``torch.rand`` per call, which is what ``F.dropout`` amounts to.
+
+Two forms the reference does not have: ``gemm="fp8"`` takes the layer's dense products in 8-bit floating point
+(``fp8.linear``; the operands are quantised, what autograd keeps of the activations is one byte a value), and
+``norm="rms"`` puts a residual stream through the model, normalised by ``norm.rms_norm``:
+
+    h = h + dropout(layer(x)),   x = relu(rms_norm(h) * weight)      between layers
+
+In front of an 8-bit layer that multiplies first the normalised rows exist in 8 bits only (``fp8.norm_linear``).
 """
 import copy
 from typing import List, Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
-from . import _lib, aggregator
+from . import _lib, aggregator, fp8
+from . import norm as rms
 from .gcn import (_FORMS, _mean_nll, input_gradient, plain_product, scored_rows, stacked_product,
                   weight_and_bias_gradient, weight_gradient)
 from .sparse_tensor import SparseTensor, _row_stride
@@ -127,25 +137,108 @@ def dropout_layernorm_relu(z, keep, scale, gamma, beta, eps) -> torch.Tensor:
     return _DropoutLayerNormRelu.apply(z, keep, scale, gamma, beta, eps)
 
 
+# ------------------------------------------------------- residual stream -> RMS norm -> ReLU
+class _ResidualRmsNormRelu(torch.autograd.Function):
+    """``h = z + residual``, ``relu(rms_norm(h))`` in one pass, the latter written into the right half of a fresh
+    ``[N, 2F]`` array (returned whole, the next layer's staged input, in front of ``h``)."""
+
+    @staticmethod
+    def forward(ctx, z, residual, weight, eps):
+        rows, feat = z.shape
+        cat = torch.empty(rows, 2 * feat, dtype=torch.float32, device=z.device)
+        _, h = rms._forward(z, weight, eps, residual, True, y=cat[:, feat:])
+        ctx.save_for_backward(z if h is None else h, weight)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return cat if h is None else (cat, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_cat, grad_h=None):
+        h, weight = ctx.saved_tensors
+        grad_z, grad_weight = grad_h, None
+        if grad_cat is not None:  # of its right half: the left half belongs to nobody
+            grad_z, grad_weight = rms._backward(grad_cat[:, h.size(1):], grad_h, h, weight, ctx.eps, True)
+        want = ctx.needs_input_grad
+        return (grad_z if want[0] else None, grad_z if want[1] else None, grad_weight if want[2] else None, None)
+
+
+def residual_rms_norm_relu(z, residual, weight, eps):
+    """(staged input ``[N, 2F]`` of the next layer, residual stream ``h``) of a layer's output ``z`` and the stream so far
+    (None in front of the first norm, where ``h`` is ``z``)."""
+    rms.check_norm(z, weight, residual)
+    if z.dim() != 2 or z.dtype != torch.float32:
+        raise RuntimeError("Input mismatch: z must be float32 [rows, feat]")
+    if residual is None:
+        return _ResidualRmsNormRelu.apply(z, None, weight, float(eps)), z
+    return _ResidualRmsNormRelu.apply(z, residual, weight, float(eps))
+
+
 # ---------------------------------------------------------------------------- the layer
+def _gradient_through_aggregation(ctx, grad_cat):
+    """Gradient ``[d/d aggregated | d/d x, direct part]`` of a staged input -> that of x in the right half, in place."""
+    fi = grad_cat.size(1) // 2
+    grad_agg = grad_cat[:, :fi]
+    if ctx.divide:
+        grad_agg.div_(ctx.graph.in_degrees)
+    # d/d x += A^T (d/d aggregated), accumulated where the direct part already lies
+    aggregator._backward(ctx, grad_agg, out=grad_cat[:, fi:], accumulate=True)
+    return grad_cat
+
+
+def _gradient_of_rows(ctx, grad_small, rows):
+    """The same for the local nodes ``rows``, into the right half of a fresh ``[N, 2 fi]`` array."""
+    fi = grad_small.size(1) // 2
+    grad_agg = grad_small[:, :fi]
+    if ctx.divide:
+        grad_agg.div_(ctx.graph.in_degrees)
+    # the gradient goes where the features were: the right half of an [N, 2 fi] array: A[rows]^T (d/d
+    # aggregated), then the direct part added onto the rows it belongs to (every row once: deterministic).
+    # The left half was scratch on the way forward: nothing depends on it, so its gradient is zero -- written
+    # as such, because autograd hands this array on (to a leaf that requires grad, or into a sum with another
+    # consumer's gradient) and uninitialised memory there could be anything, NaN included.
+    grad_cat = torch.empty(ctx.nodes, 2 * fi, dtype=torch.float32, device=grad_small.device)
+    grad_cat[:, :fi].zero_()
+    target = grad_cat[:, fi:]
+    aggregator._backward(ctx, grad_agg, out=target, accumulate=False)
+    target.index_add_(0, rows, grad_small[:, fi:])
+    return grad_cat
+
+
+def _stage_aggregated(ctx, graph, cat, layer, num_bits, is_pre_delay, is_training, normalize):
+    """The aggregated (and degree-normalised) rows of a staged input's right half, into its left half."""
+    fi = cat.size(1) // 2
+    agg = cat[:, :fi]
+    aggregator._forward(ctx, graph, aggregator._DenseFeatures(cat[:, fi:]), layer, num_bits, is_pre_delay, is_training,
+                        out=agg)
+    ctx.divide = bool(normalize) and not getattr(graph, "in_degrees_folded", False)
+    if ctx.divide:
+        agg.div_(graph.in_degrees)  # sageconv.py:80-82
+    else:
+        # the library wrote the left half behind autograd's back: an (empty) in-place op bumps the
+        # array's version, so that an earlier call that kept this same array for its backward
+        # fails loudly there instead of reading rows that are no longer its own
+        cat[:0].zero_()
+
+
+def _rows_side_by_side(ctx, graph_rows, cat, layer, num_bits, is_pre_delay, is_training, normalize, rows):
+    """``[A[rows] x / deg[rows] | x[rows]]`` of a staged input."""
+    x = cat[:, cat.size(1) // 2:]
+    agg = aggregator._forward(ctx, graph_rows, aggregator._DenseFeatures(x), layer, num_bits, is_pre_delay, is_training)
+    ctx.divide = bool(normalize) and not getattr(graph_rows, "in_degrees_folded", False)
+    if ctx.divide:
+        agg.div_(graph_rows.in_degrees)
+    ctx.nodes = cat.size(0)
+    return torch.cat([agg, x.index_select(0, rows)], dim=1)  # [len(rows), 2 fi]
+
+
 class _SageConv(torch.autograd.Function):
     """``[A x / deg | x] @ W + bias`` on a staged input ``cat`` (right half = x; the left half is
     overwritten with the aggregated rows and kept for the weight gradient)."""
 
     @staticmethod
     def forward(ctx, graph, cat, weight, bias, layer, num_bits, is_pre_delay, is_training, normalize, form=0):
-        fi = cat.size(1) // 2
-        x, agg = cat[:, fi:], cat[:, :fi]
-        aggregator._forward(ctx, graph, aggregator._DenseFeatures(x), layer, num_bits, is_pre_delay, is_training,
-                            out=agg)
-        ctx.divide = bool(normalize) and not getattr(graph, "in_degrees_folded", False)
-        if ctx.divide:
-            agg.div_(graph.in_degrees)  # sageconv.py:80-82
-        else:
-            # the library wrote the left half behind autograd's back: an (empty) in-place op bumps the
-            # array's version, so that an earlier call that kept this same array for its backward
-            # fails loudly there instead of reading rows that are no longer its own
-            cat[:0].zero_()
+        _stage_aggregated(ctx, graph, cat, layer, num_bits, is_pre_delay, is_training, normalize)
         out = stacked_product(cat, weight, bias, form)
         ctx.save_for_backward(cat, weight)
         ctx.has_bias = bias is not None
@@ -172,12 +265,8 @@ class _SageConv(torch.autograd.Function):
         elif want_b:
             grad_b = g.sum(dim=0)
         if ctx.needs_input_grad[1]:
-            grad_cat = input_gradient(g, weight, ctx.form)  # [N, 2 fi]: d/d aggregated | d/d x (direct part)
-            grad_agg = grad_cat[:, :fi]
-            if ctx.divide:
-                grad_agg.div_(ctx.graph.in_degrees)
-            # d/d x += A^T (d/d aggregated), accumulated where the direct part already lies
-            aggregator._backward(ctx, grad_agg, out=grad_cat[:, fi:], accumulate=True)
+            # [N, 2 fi]: d/d aggregated | d/d x (direct part)
+            grad_cat = _gradient_through_aggregation(ctx, input_gradient(g, weight, ctx.form))
         return None, grad_cat, grad_w, grad_b, None, None, None, None, None, None
 
 
@@ -188,19 +277,11 @@ class _SageConvRows(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, graph_rows, cat, weight, bias, layer, num_bits, is_pre_delay, is_training, normalize, rows, form=0):
-        fi = cat.size(1) // 2
-        x = cat[:, fi:]
-        agg = aggregator._forward(ctx, graph_rows, aggregator._DenseFeatures(x), layer, num_bits, is_pre_delay,
-                                  is_training)
-        ctx.divide = bool(normalize) and not getattr(graph_rows, "in_degrees_folded", False)
-        if ctx.divide:
-            agg.div_(graph_rows.in_degrees)
-        small = torch.cat([agg, x.index_select(0, rows)], dim=1)  # [len(rows), 2 fi]
+        small = _rows_side_by_side(ctx, graph_rows, cat, layer, num_bits, is_pre_delay, is_training, normalize, rows)
         out = stacked_product(small, weight, bias, form)
         ctx.save_for_backward(small, weight, rows)
         ctx.has_bias = bias is not None
         ctx.form = form
-        ctx.nodes = cat.size(0)
         return out
 
     @staticmethod
@@ -221,20 +302,8 @@ class _SageConvRows(torch.autograd.Function):
         elif want_b:
             grad_b = g.sum(dim=0)
         if ctx.needs_input_grad[1]:
-            grad_small = input_gradient(g, weight, ctx.form)  # [len(rows), 2 fi]: d/d aggregated | d/d x[rows] (direct part)
-            grad_agg = grad_small[:, :fi]
-            if ctx.divide:
-                grad_agg.div_(ctx.graph.in_degrees)
-            # the gradient goes where the features were: the right half of an [N, 2 fi] array: A[rows]^T (d/d
-            # aggregated), then the direct part added onto the rows it belongs to (every row once: deterministic).
-            # The left half was scratch on the way forward: nothing depends on it, so its gradient is zero -- written
-            # as such, because autograd hands this array on (to a leaf that requires grad, or into a sum with another
-            # consumer's gradient) and uninitialised memory there could be anything, NaN included.
-            grad_cat = torch.empty(ctx.nodes, 2 * fi, dtype=torch.float32, device=g.device)
-            grad_cat[:, :fi].zero_()
-            target = grad_cat[:, fi:]
-            aggregator._backward(ctx, grad_agg, out=target, accumulate=False)
-            target.index_add_(0, rows, grad_small[:, fi:])
+            # [len(rows), 2 fi]: d/d aggregated | d/d x[rows] (direct part)
+            grad_cat = _gradient_of_rows(ctx, input_gradient(g, weight, ctx.form), rows)
         return None, grad_cat, grad_w, grad_b, None, None, None, None, None, None, None
 
 
@@ -297,6 +366,60 @@ class _SageConvLinearFirst(torch.autograd.Function):
         return None, grad_x, grad_w, grad_b, None, None, None, None, None, None
 
 
+# ------------------------------------------------------------------- the layer in 8 bits
+class _StagedRows(torch.autograd.Function):
+    """The left operand ``[A x / deg | x]`` of the layer's product by itself: the staged input with its left half filled.
+    ``fp8.linear`` behind it keeps the quantised codes, so nobody keeps the array."""
+
+    @staticmethod
+    def forward(ctx, graph, cat, layer, num_bits, is_pre_delay, is_training, normalize):
+        _stage_aggregated(ctx, graph, cat, layer, num_bits, is_pre_delay, is_training, normalize)
+        return cat.detach()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_cat):
+        # (the product's input gradient, made for this pass alone: nobody else reads it)
+        return None, _gradient_through_aggregation(ctx, grad_cat), None, None, None, None, None
+
+
+class _RestrictedRows(torch.autograd.Function):
+    """The same for the local nodes ``rows``, ``[len(rows), 2 fi]``."""
+
+    @staticmethod
+    def forward(ctx, graph_rows, cat, layer, num_bits, is_pre_delay, is_training, normalize, rows):
+        small = _rows_side_by_side(ctx, graph_rows, cat, layer, num_bits, is_pre_delay, is_training, normalize, rows)
+        ctx.save_for_backward(rows)
+        return small
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_small):
+        (rows,) = ctx.saved_tensors
+        return None, _gradient_of_rows(ctx, grad_small, rows), None, None, None, None, None, None
+
+
+class _AggregateProducts(torch.autograd.Function):
+    """``A left / deg + right`` of ``[left | right]``: the layer behind its product, for a layer that multiplies first."""
+
+    @staticmethod
+    def forward(ctx, graph, both, layer, num_bits, is_pre_delay, is_training, normalize):
+        fo = both.size(1) // 2
+        ctx.divide = bool(normalize) and not getattr(graph, "in_degrees_folded", False)
+        agg = aggregator._forward(ctx, graph, aggregator._DenseFeatures(both[:, :fo]), layer, num_bits, is_pre_delay,
+                                  is_training)
+        return torch.addcdiv(both[:, fo:], agg, graph.in_degrees) if ctx.divide else agg.add_(both[:, fo:])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        fo = g.size(1)
+        grad_both = torch.empty(g.size(0), 2 * fo, dtype=torch.float32, device=g.device)
+        aggregator._backward(ctx, g / ctx.graph.in_degrees if ctx.divide else g, out=grad_both[:, :fo])
+        grad_both[:, fo:] = g
+        return None, grad_both, None, None, None, None, None
+
+
 class _LinearView:
     """What the reference's ``lin_neigh`` / ``lin_self`` expose: ``weight`` as ``[out, in]`` -- here
     a view of the layer's stacked weight."""
@@ -323,9 +446,9 @@ class DistSAGEConvGrad(torch.nn.Module):
         # gemm "bf16x3": all of the layer's dense products in libgnnagg's kernels with every fp32 operand as three bf16
         # pieces (fp32 accuracy on the bf16 matrix units); "fp32": the stacked product and the input-gradient product
         # likewise (plain products, for which that form is the fastest fp32-accurate one), the weight gradients with the
-        # fp32 matrix instruction
-        if gemm not in ("fp32", "bf16x3"):
-            raise ValueError("gemm must be 'fp32' or 'bf16x3'")
+        # fp32 matrix instruction; "fp8": the products of ``fp8.linear``, operands in 8 bits with a scale per block of 128
+        if gemm not in ("fp32", "bf16x3", "fp8"):
+            raise ValueError("gemm must be 'fp32', 'bf16x3' or 'fp8'")
         self.gemm = gemm
         self.in_channels = in_channels
         self.out_channels = out_channels
@@ -364,6 +487,18 @@ class DistSAGEConvGrad(torch.nn.Module):
             self.weight[:self.in_channels] = lin_neigh_weight.t()
             self.weight[self.in_channels:] = lin_self_weight.t()
 
+    def product_weight(self) -> torch.Tensor:
+        """``[W_n | W_s]``, the weight of a layer that multiplies first, for one product over both."""
+        return torch.cat([self.weight[:self.in_channels], self.weight[self.in_channels:]], dim=1)
+
+    def product_bias(self) -> Optional[torch.Tensor]:
+        return None if self.bias is None else F.pad(self.bias, (self.out_channels, 0))
+
+    def aggregate_products(self, graph, both: torch.Tensor, layer: int) -> torch.Tensor:
+        """The layer's output from its products ``[x W_n | x W_s + bias]``."""
+        return _AggregateProducts.apply(graph, both, layer, self.num_bits, self.is_pre_delay, self.training,
+                                        self.normalize)
+
     def forward(self, graph, local_nodes_feat: torch.Tensor, layer: int,
                 rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``local_nodes_feat``: ``[N, in_channels]`` features (staged here, one copy) or an
@@ -379,6 +514,9 @@ class DistSAGEConvGrad(torch.nn.Module):
                                    % (self.in_channels, 2 * self.in_channels, width))
             if not local_nodes_feat.is_cuda or local_nodes_feat.dtype != torch.float32:
                 raise RuntimeError("Input mismatch: the features must be a float32 GPU (HIP) tensor")
+            if self.gemm == "fp8":
+                x = local_nodes_feat[:, width - self.in_channels:]
+                return self.aggregate_products(graph, fp8.linear(x, self.product_weight(), self.product_bias()), layer)
             return _SageConvLinearFirst.apply(graph, local_nodes_feat, self.weight, self.bias, layer, self.num_bits,
                                               self.is_pre_delay, self.training, self.normalize, _FORMS[self.gemm])
         if width == self.in_channels:
@@ -394,26 +532,39 @@ class DistSAGEConvGrad(torch.nn.Module):
             raise RuntimeError("Input mismatch: the staged input must be a contiguous float32 GPU (HIP) tensor")
         if rows is not None:
             graph_rows = aggregator.restrict_output_rows(graph, rows, self.is_pre_delay)
+            if self.gemm == "fp8":
+                small = _RestrictedRows.apply(graph_rows, cat, layer, self.num_bits, self.is_pre_delay, self.training,
+                                              self.normalize, rows)
+                return fp8.linear(small, self.weight, self.bias)
             return _SageConvRows.apply(graph_rows, cat, self.weight, self.bias, layer, self.num_bits, self.is_pre_delay,
                                        self.training, self.normalize, rows, _FORMS[self.gemm])
+        if self.gemm == "fp8":
+            staged = _StagedRows.apply(graph, cat, layer, self.num_bits, self.is_pre_delay, self.training, self.normalize)
+            return fp8.linear(staged, self.weight, self.bias)
         return _SageConv.apply(graph, cat, self.weight, self.bias, layer, self.num_bits, self.is_pre_delay,
                                self.training, self.normalize, _FORMS[self.gemm])
 
 
 # ---------------------------------------------------------------------------- the model
 class DistSAGE(torch.nn.Module):
-    """DistSAGE.py:13-69: ``num_layers`` SAGE layers, LayerNorm after all but the last."""
+    """DistSAGE.py:13-69: ``num_layers`` SAGE layers, LayerNorm after all but the last.  ``norm="rms"``: a residual
+    stream over the hidden layers and RMS norms in their place.  ``gemm``: the form of the dense products, see
+    ``DistSAGEConvGrad``."""
 
     def __init__(self, in_channels, hidden_channels, out_channels, num_layers=3, dropout=0.5, num_bits=32,
-                 is_pre_delay=False, linear_first_when_narrowing=False, gemm="fp32"):
+                 is_pre_delay=False, linear_first_when_narrowing=False, gemm="fp32", norm="layer"):
         super().__init__()
+        if norm not in ("layer", "rms"):
+            raise ValueError("norm must be 'layer' or 'rms'")
+        self.norm = norm
+        make_norm = torch.nn.LayerNorm if norm == "layer" else rms.RmsNorm
         self.convs = torch.nn.ModuleList()
         self.norms = torch.nn.ModuleList()
         self.convs.append(DistSAGEConvGrad(in_channels, hidden_channels, num_bits, is_pre_delay, gemm=gemm))
-        self.norms.append(torch.nn.LayerNorm(hidden_channels))
+        self.norms.append(make_norm(hidden_channels))
         for _ in range(num_layers - 2):
             self.convs.append(DistSAGEConvGrad(hidden_channels, hidden_channels, num_bits, is_pre_delay, gemm=gemm))
-            self.norms.append(torch.nn.LayerNorm(hidden_channels))
+            self.norms.append(make_norm(hidden_channels))
         self.convs.append(DistSAGEConvGrad(hidden_channels, out_channels, num_bits, is_pre_delay, gemm=gemm))
         if linear_first_when_narrowing:  # a layer with fewer outputs than inputs aggregates its outputs
             for conv in self.convs:
@@ -434,15 +585,33 @@ class DistSAGE(torch.nn.Module):
         model/DistSAGE.py:69 (a caller that scores a subset of the nodes applies it to those rows).
         ``last_rows`` (local node ids): evaluate the last layer for those nodes only and return
         ``[len(last_rows), out_channels]``."""
+        stream = both = None
         for i, conv in enumerate(self.convs[:-1]):
-            z = conv(graph, nodes_feats, i)
+            z = conv(graph, nodes_feats, i) if both is None else conv.aggregate_products(graph, both, i)
             keep, scale = None, 1.0
             if self.training and self.dropout > 0.0:
                 keep = masks[i] if masks is not None else torch.rand_like(z) >= self.dropout
                 scale = 1.0 / (1.0 - self.dropout)
             norm = self.norms[i]
-            nodes_feats = dropout_layernorm_relu(z, keep, scale, norm.weight, norm.bias, norm.eps)
-        out = self.convs[-1](graph, nodes_feats, len(self.convs) - 1, last_rows)
+            if self.norm == "layer":
+                nodes_feats = dropout_layernorm_relu(z, keep, scale, norm.weight, norm.bias, norm.eps)
+                continue
+            if keep is not None:
+                z = z * keep * scale
+            after = self.convs[i + 1]
+            both = None
+            if after.gemm == "fp8" and after.linear_first:  # the normalised rows exist in 8 bits only
+                both, stream = fp8.norm_linear(z, norm.weight, norm.eps, after.product_weight(), after.product_bias(),
+                                               residual=stream, relu=True)
+            else:
+                nodes_feats, stream = residual_rms_norm_relu(z, stream, norm.weight, norm.eps)
+        last = len(self.convs) - 1
+        if both is not None:
+            if last_rows is not None:
+                raise RuntimeError("a layer that multiplies first has no row-restricted form")
+            out = self.convs[-1].aggregate_products(graph, both, last)
+        else:
+            out = self.convs[-1](graph, nodes_feats, last, last_rows)
         return F.log_softmax(out, dim=1) if log_probs else out
 
 
