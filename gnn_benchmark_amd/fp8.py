@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib
+from . import _lib, ext
 
 BLOCK = 128
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -100,21 +100,11 @@ class QuantizedWeight:
 
 def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     """fp32 or bf16 [rows, width] -> the 8-bit format.  No gradient (``linear`` has one)."""
-    _refuse_grad(x)
-    return _quantize_rows(x)
+    return QuantizedRows(*ext.train_ops().quantize_rows(x), x.size(1))
 
 
 def _quantize_rows(x: torch.Tensor) -> QuantizedRows:
-    check_gpu(x, "x")
-    code = dtype_code(x.dtype, "x")
-    if x.dim() != 2 or x.size(1) == 0:
-        raise RuntimeError("Input mismatch: x must be [rows, width] with a width above zero")
-    x = as_rows(x)
-    q = QuantizedRows.empty(x.size(0), x.size(1), x.device)
-    with _lib.on_device(x.device):
-        _lib.check(_lib.lib().gnnagg_fp8_quantize_rows(address(x), row_stride(x), address(q.codes), address(q.scales),
-                                                       x.size(0), x.size(1), code, _lib.raw_stream(x.device)))
-    return q
+    return QuantizedRows(*ext.train_ops().quantize_rows_forward(x), x.size(1))
 
 
 def quantize_weight(w: torch.Tensor, for_gradient: bool = False) -> QuantizedWeight:
@@ -155,46 +145,14 @@ def product(x: QuantizedRows, weight: QuantizedWeight, bias: Optional[torch.Tens
     """``x @ weight (+ bias)`` of 8-bit operands, [rows, n] in ``out_dtype`` (fp32 accumulation, one rounding).
     ``input_gradient``: ``x @ weight^T``, [rows, k], from the codes by input.  ``out``: an array of that shape with
     contiguous rows (a column block of a wider one is fine) to write into.  No gradient (``linear`` has one)."""
-    _refuse_grad(bias, out)
-    return _product(x, weight, bias, out_dtype, out, input_gradient)
+    return ext.train_ops().product(x.codes, x.scales, x.cols, weight.codes_by_input if input_gradient else weight.codes,
+                                   weight.scales, weight.k, weight.n, bias, out_dtype, out, input_gradient)
 
 
-def _product(x, weight, bias, out_dtype, out=None, input_gradient=False):
-    x.check("x")
-    rows, device = x.codes.size(0), x.codes.device
-    inner, wide = (weight.n, weight.k) if input_gradient else (weight.k, weight.n)
-    codes, scales = weight.codes_by_input if input_gradient else weight.codes, weight.scales
-    if codes is None:
-        raise RuntimeError("Input mismatch: the weight was quantised without the codes this product reads")
-    check_gpu(codes, "the weight", device)
-    check_gpu(scales, "the weight's scales", device)
-    if x.cols != inner:
-        raise RuntimeError(f"Input mismatch: x has {x.cols} columns, the weight's inner width is {inner}")
-    if (codes.dtype != torch.float8_e4m3fn or tuple(codes.shape) != (wide, padded(inner)) or not codes.is_contiguous()
-            or codes.data_ptr() % 16 != 0):
-        raise RuntimeError("Input mismatch: the weight must hold contiguous, 16-byte aligned float8_e4m3fn codes "
-                           "[outputs, inner width rounded up to 128]")
-    if (scales.dtype != torch.float8_e8m0fnu
-            or tuple(scales.shape) != (padded(weight.k) // BLOCK, padded(weight.n) // BLOCK)):
-        raise RuntimeError("Input mismatch: the weight must hold float8_e8m0fnu scales [k blocks, n blocks]")
-    code = dtype_code(out_dtype if out is None else out.dtype, "out")
-    if bias is not None:
-        check_gpu(bias, "the bias", device)
-        if bias.numel() != wide:
-            raise RuntimeError(f"Input mismatch: the bias holds {bias.numel()} values for {wide} outputs")
-        bias = bias.detach().reshape(-1).float().contiguous()
-    if out is None:
-        out = torch.empty(rows, wide, dtype=out_dtype, device=device)
-    else:
-        check_gpu(out, "out", device)
-        if tuple(out.shape) != (rows, wide) or as_rows(out) is not out:
-            raise RuntimeError("Input mismatch: out must be [rows, outputs] with contiguous rows")
-    stride_k, stride_n = scales.stride()[::-1] if input_gradient else scales.stride()
-    with _lib.on_device(device):
-        _lib.check(_lib.lib().gnnagg_fp8_product(
-            address(x.codes), address(x.scales), address(codes), address(scales), stride_k, stride_n, address(bias),
-            address(out), row_stride(out), code, rows, inner, wide, _lib.raw_stream(device)))
-    return out
+def _product(x, weight, bias, out_dtype, input_gradient=False):
+    return ext.train_ops().product_forward(
+        x.codes, x.scales, x.cols, weight.codes_by_input if input_gradient else weight.codes, weight.scales, weight.k,
+        weight.n, bias, out_dtype, None, input_gradient)
 
 
 def weight_gradient(x: QuantizedRows, g: torch.Tensor, with_bias: bool = False):
@@ -325,9 +283,6 @@ def norm_linear(x: torch.Tensor, norm_weight: torch.Tensor, eps: float, w: torch
                 relu: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """``linear(norm.rms_norm(x + residual), w, bias)`` with the normalised rows written in 8 bits by the norm itself:
     (result, h) with ``h = x + residual`` the residual stream (``x`` itself without a residual)."""
-    from . import norm
-
-    norm.check_norm(x, norm_weight, residual)
     _check_linear(x, w, bias)
     if residual is None:
         return _NormLinear.apply(x, None, norm_weight, float(eps), bool(relu), w, bias), x

@@ -7,55 +7,18 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib
-from .fp8 import QuantizedRows, _refuse_grad, address, as_rows, check_gpu, dtype_code, row_stride
-
-
-def check_norm(x, weight, residual) -> None:
-    check_gpu(x, "x")
-    check_gpu(weight, "the norm's weight", x.device)
-    dtype_code(x.dtype, "x")
-    if x.dim() < 1 or weight.dim() != 1 or weight.numel() != x.size(-1):
-        raise RuntimeError("Input mismatch: the norm's weight must hold one value per column of x")
-    if weight.dtype != torch.float32 and weight.dtype != x.dtype:
-        raise RuntimeError("Input mismatch: the norm's weight must be float32 or of x's type")
-    if residual is not None:
-        check_gpu(residual, "the residual", x.device)
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise RuntimeError("Input mismatch: the residual must have x's shape and type")
-
-
-def _operands(x, weight, residual):
-    """What both forward forms pass: rows of x and of the residual, the weight, a fresh h (x's shape) or None."""
-    rows = as_rows(x)
-    res = None if residual is None else as_rows(residual)
-    h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    return rows, res, weight.detach().contiguous(), h
+from . import _lib, ext
+from .fp8 import QuantizedRows, address, as_rows, dtype_code, row_stride
 
 
 def _forward(x, weight, eps, residual, relu, y=None):
-    rows, res, w, h = _operands(x, weight, residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if y is None else y
-    yr = y.view(-1, x.size(-1)) if y.dim() != 2 else y
-    with _lib.on_device(x.device):
-        _lib.check(_lib.lib().gnnagg_rms_norm(
-            address(rows), row_stride(rows), address(res), 0 if res is None else row_stride(res), address(w),
-            dtype_code(w.dtype, "the norm's weight"), float(eps), 1 if relu else 0, address(h),
-            0 if h is None else x.size(-1), address(yr), row_stride(yr), rows.size(0), rows.size(1),
-            dtype_code(x.dtype, "x"), _lib.raw_stream(x.device)))
-    return y, h
+    """(y, h or None)"""
+    return ext.train_ops().rms_norm(x, weight, eps, residual, relu, y)
 
 
 def _forward_fp8(x, weight, eps, residual, relu):
-    rows, res, w, h = _operands(x, weight, residual)
-    q = QuantizedRows.empty(rows.size(0), rows.size(1), x.device)
-    with _lib.on_device(x.device):
-        _lib.check(_lib.lib().gnnagg_rms_norm_fp8(
-            address(rows), row_stride(rows), address(res), 0 if res is None else row_stride(res), address(w),
-            dtype_code(w.dtype, "the norm's weight"), float(eps), 1 if relu else 0, address(h),
-            0 if h is None else x.size(-1), address(q.codes), address(q.scales), rows.size(0), rows.size(1),
-            dtype_code(x.dtype, "x"), _lib.raw_stream(x.device)))
-    return q, (x if h is None else h)
+    codes, scales, h = ext.train_ops().rms_norm_fp8_forward(x, weight, eps, residual, relu)
+    return QuantizedRows(codes, scales, x.size(-1)), (x if h is None else h)
 
 
 def _backward(grad_y, grad_h, h, weight, eps, relu):
@@ -105,7 +68,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     """``(y, h)`` of x [..., width]: ``h = x + residual`` (rounded to x's type; ``x`` itself without a residual) and
     ``y`` its RMS norm times ``weight``, through a ReLU where asked for.  Differentiable in x, the residual and the
     weight; the gradient of ``h``, where it is used further, is added inside the backward pass."""
-    check_norm(x, weight, residual)
+    if not torch.is_grad_enabled():
+        y, h = _forward(x, weight, eps, residual, relu)
+        return y, (x if h is None else h)
     if residual is None:
         return _RmsNorm.apply(x, None, weight, float(eps), bool(relu)), x
     return _RmsNorm.apply(x, residual, weight, float(eps), bool(relu))
@@ -115,9 +80,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
                  relu: bool = False) -> Tuple[QuantizedRows, torch.Tensor]:
     """``rms_norm`` with ``y`` in the 8-bit format (``fp8.QuantizedRows``; leading dimensions become rows), quantised
     from its fp32 value.  No gradient: ``fp8.norm_linear`` is the differentiable norm in front of a product."""
-    check_norm(x, weight, residual)
-    _refuse_grad(x, weight, residual)
-    return _forward_fp8(x, weight, eps, residual, relu)
+    codes, scales, h = ext.train_ops().rms_norm_fp8(x, weight, eps, residual, relu)
+    return QuantizedRows(codes, scales, x.size(-1)), (x if h is None else h)
 
 
 class RmsNorm(torch.nn.Module):

@@ -10,35 +10,12 @@ neighbours with the odds of the distance, because a step at ``beta2 = 0.999`` mo
 and rounding to nearest would never let it move.  The random bits come from a hash of (seed, tensor, step, element): the
 same calls give the same bits, on every rank.
 """
-import ctypes
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
-from . import _lib
-from .fp8 import BLOCK, address, dtype_code
-
-_FIELDS = 8  # words of a gnnagg_adamw_tensor
-
-
-def _same(tensors: Sequence[torch.Tensor], dtypes, device, what: str, count: int) -> torch.dtype:
-    """The one type of ``count`` contiguous tensors on the device.  (Mapped over the list: a Python loop over hundreds of
-    tensors takes longer than their update.)"""
-    if len(tensors) != count:
-        raise RuntimeError(f"Input mismatch: {len(tensors)} {what} for {count} parameters")
-    kinds = {t.dtype for t in tensors}
-    if len(kinds) != 1 or not kinds <= dtypes:
-        raise RuntimeError(f"Input mismatch: {what} must all have one type, of " + ", ".join(sorted(map(str, dtypes))))
-    if set(map(torch.Tensor.get_device, tensors)) != {device.index}:
-        raise RuntimeError(f"Input mismatch: {what} must be on the parameters' GPU (HIP) device")
-    if not all(map(torch.Tensor.is_contiguous, tensors)):
-        raise RuntimeError(f"Input mismatch: {what} must be contiguous")
-    return kinds.pop()
-
-
-def _sizes(tensors) -> list:
-    return list(map(torch.Tensor.numel, tensors))
-
+from . import ext
+from .fp8 import BLOCK
 
 _FLOATS = {torch.float32, torch.bfloat16}
 
@@ -55,72 +32,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     rounded).  Gradients: all fp32 or all bf16.  States: fp32 ``exp_avgs`` / ``exp_avg_sqs``, or float8_e4m3fn codes of m
     and sqrt(v) with ``exp_avg_scales`` / ``exp_avg_sq_scales`` (float8_e8m0fnu, one for each 128 elements).  ``lr``: a
     number, or an fp32 scalar on the device that is read when the step runs.  No tensor that is written may overlap another
-(the same one twice is refused).  ``first``: number of the first tensor for
+(that is refused).  ``first``: number of the first tensor for
     the 8-bit states' random bits, where a list is split over calls."""
-    count = len(params)
-    if count == 0:
-        return
-    device = params[0].device
-    if device.type != "cuda":
-        raise RuntimeError("Input mismatch: parameters must be GPU (HIP) tensors")
-    with torch.no_grad():
-        param_dtype = _same(params, _FLOATS, device, "parameters", count)
-        grad_dtype = _same(grads, _FLOATS, device, "gradients", count)
-        state_dtype = _same(exp_avgs, {torch.float32, torch.float8_e4m3fn}, device, "states", count)
-        _same(exp_avg_sqs, {state_dtype}, device, "states", count)
-        lists = [params, grads, exp_avgs, exp_avg_sqs]
-        sizes = _sizes(params)
-        for tensors, what in ((grads, "gradient"), (exp_avgs, "state"), (exp_avg_sqs, "state")):
-            if _sizes(tensors) != sizes:
-                raise RuntimeError(f"Input mismatch: a {what} has another size than its parameter")
-        eight = state_dtype == torch.float8_e4m3fn
-        if eight:
-            if exp_avg_scales is None or exp_avg_sq_scales is None:
-                raise RuntimeError("Input mismatch: states in 8 bits need their scales")
-            blocks = [-(-n // BLOCK) for n in sizes]
-            for scales in (exp_avg_scales, exp_avg_sq_scales):
-                _same(scales, {torch.float8_e8m0fnu}, device, "scales", count)
-                if _sizes(scales) != blocks:
-                    raise RuntimeError("Input mismatch: scales hold one value for each 128 elements of their state")
-            lists += [exp_avg_scales, exp_avg_sq_scales]
-        elif exp_avg_scales is not None or exp_avg_sq_scales is not None:
-            raise RuntimeError("Input mismatch: states in 32 bits have no scales")
-        if param_dtype == torch.bfloat16:
-            if masters is None:
-                raise RuntimeError("Input mismatch: bfloat16 parameters need their float32 masters")
-            _same(masters, {torch.float32}, device, "masters", count)
-            if _sizes(masters) != sizes:
-                raise RuntimeError("Input mismatch: a master has another size than its parameter")
-        elif masters is not None:
-            raise RuntimeError("Input mismatch: float32 parameters have no masters")
-        if (steps.device != device or steps.dtype != torch.int32 or steps.dim() != 1 or steps.numel() != count
-                or not steps.is_contiguous()):
-            raise RuntimeError("Input mismatch: steps must be contiguous int32 [parameters] on their device")
-        lr_tensor = None
-        if isinstance(lr, torch.Tensor):
-            if lr.device == device:
-                if lr.dtype != torch.float32 or lr.numel() != 1:
-                    raise RuntimeError("Input mismatch: a learning rate on the device must be a float32 scalar")
-                lr_tensor, lr = lr, 0.0
-            else:
-                lr = float(lr)
-        records = (ctypes.c_uint64 * (_FIELDS * count))()
-        written = []
-        for at, tensors in enumerate(lists + ([] if masters is None else [masters])):
-            addresses = list(map(torch.Tensor.data_ptr, tensors))
-            records[at if tensors is not masters else 6::_FIELDS] = addresses
-            if tensors is not grads:
-                written += addresses
-        written = [a for a in written if a]  # (an empty tensor has none)
-        if len(set(written)) != len(written):
-            raise RuntimeError("Input mismatch: the same memory twice among parameters, states and masters")
-        records[7::_FIELDS] = sizes
-        with _lib.on_device(device):
-            _lib.check(_lib.lib().gnnagg_adamw_step(
-                ctypes.cast(records, ctypes.POINTER(_lib.AdamwTensor)), count, address(steps),
-                dtype_code(param_dtype, "parameters"), dtype_code(grad_dtype, "gradients"), 8 if eight else 32, float(lr),
-                address(lr_tensor), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
-                int(seed) & 0xFFFFFFFF, int(first), _lib.raw_stream(device)))
+    ext.train_ops().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas[0], betas[1], eps, weight_decay, masters,
+                               exp_avg_scales, exp_avg_sq_scales, seed & 0xFFFFFFFF, first)
 
 
 class AdamW(torch.optim.Optimizer):
