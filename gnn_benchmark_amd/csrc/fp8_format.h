@@ -158,11 +158,13 @@ __device__ __forceinline__ f32x4 rounded(const bf16_t *, const f32x4 v) {
 // way to registers, which takes the point out of asking for them early.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// keeps an address that is the same for the whole wave in scalar registers
+// Keeps an address that is the same for the whole wave in scalar registers.  (Said to be global memory's on the way through:
+// behind the asm the compiler would not know, and a flat load also counts as an LDS access, which every barrier waits for.)
 template <typename T>
 __device__ __forceinline__ const T *scalar(const T *p) {
-    asm volatile("" : "+s"(p));
-    return p;
+    const __attribute__((address_space(1))) T *global = (const __attribute__((address_space(1))) T *)p;
+    asm volatile("" : "+s"(global));
+    return (const T *)global;
 }
 
 // host: may rows at p with this stride and width be moved four values at a time?

@@ -34,18 +34,20 @@ struct WgradArgs {
     const uint8_t *x, *x_scales;
     const void *g;
     float *out, *bias_out;     // slice 0's result; slice s lies s * k * n (s * n) floats behind
+    uint8_t *g_codes, *g_scales;   // where g's rows go in the 8-bit format, or null
     int64_t g_stride, rows, rows_per_slice, k, n;
     int blocks;                // of 128 along x's rows
     int tiles_n;
 };
 
-// Byte offset of 16-byte piece q (eight rows) of column c in a staged operand.  64 bytes a column; columns are exchanged
-// inside their group of four and pieces inside their column.  A 16-byte LDS access takes its lanes in fours of which groups
-// 0, 3, 5, 6 (and 1, 2, 4, 7) of a half-wave go together; with this order both the writes (column 4 lane + const) and the
-// reads (column lane + const) of such 16 lanes fall on 16 different groups of banks.
+// Byte offset of 16-byte piece q (eight rows) of column c in a staged operand: four columns a 256-byte line, the line's 16
+// pieces in an order of its own.  A 16-byte LDS access takes its lanes in fours of which groups 0, 3, 5, 6 (and 1, 2, 4, 7)
+// of a half-wave go together; with u0..u5 the bits of the line's number these orders let such 16 lanes fall on 16 different
+// pieces' banks whether they hold consecutive columns (reads), every fourth or every eighth (writes).
 __device__ __forceinline__ int staged(int c, int q) {
-    const int u = c >> 2, v = c >> 4;
-    return (c ^ (u & 3)) * (2 * kRows) + 16 * (q ^ ((u ^ (3 * (v & 1)) ^ (v >> 1)) & 3));
+    const int u = c >> 2;
+    const int order = (u >> 1 & 1) | (u >> 1 & 2) | (u >> 2 & 4) | ((u ^ u >> 5) & 1) << 3;
+    return 256 * u + 16 * ((4 * (c & 3) + q) ^ order);
 }
 
 // eight rows of four columns, two bf16 values a word -> four pieces
@@ -71,192 +73,316 @@ __device__ __forceinline__ uint32_t word(bf16x2_t h) {
     return x.u;
 }
 
-// What a thread brings of one operand: four neighbouring columns of eight rows, in registers as they lie in memory (no
-// conversion, so no wait, before they are written to LDS).  The rows are the same for a whole wave: scalar addresses.
+struct Place {                 // of a block and a wave in the result and in the rows
+    int64_t k0, n0, begin, end;
+    int wk, wn, quarter, lane; // quarter: of the four waves that bring the same operand
+    bool live, sums, rows;     // the wave's part of the result lies inside the matrix; it adds up g's columns; hands on its
+                               // rows in 8 bits
+};
+
+// What a thread brings of one operand: eight rows of kCols neighbouring columns, in registers as they lie in memory (no
+// conversion, so no wait, before they are written to LDS).  The loads are as wide as memory allows: a load costs the
+// address and return paths much the same whatever its width, and with 4 bytes of x and 8 of g a lane these paths, not the
+// matrix units, set the pace (8192 rows, 4096 x 4096, bf16 g: 0.33 ms).  With eight columns a thread two of the four waves
+// hold a whole stage, and the pairs take turns.
 struct XRun {
     static constexpr bool kIsX = true;
-    uint32_t code[8];
-    int exponent[8];
+    static constexpr int kCols = 8;
+    uint2 code[8];
+    int exponent;                    // of row lane % 8 and this lane's block: a load for all rows, handed round below
     const uint8_t *codes, *scales;   // of the operand's first row
     uint32_t column, block;          // this lane's
+    int row, oct;                    // lane % 8; which eight rows of a stage
     int64_t pitch, blocks;           // bytes from row to row of either
 
-    __device__ __forceinline__ XRun(const WgradArgs &p, int64_t k0, int64_t, int quad) {
+    __device__ __forceinline__ XRun(const WgradArgs &p, const Place &w) {
         blocks = p.blocks;
         pitch = blocks * kBlock8;
-        const int64_t c = k0 + 4 * quad < pitch ? k0 + 4 * quad : pitch - 4;  // (past the matrix: its results are not stored)
-        column = (uint32_t)c;
-        block = (uint32_t)(c / kBlock8);
+        const int64_t c = w.k0 + 8 * (w.lane % 32);
+        column = (uint32_t)(c < pitch ? c : pitch - 8);   // (past the matrix: its results are not stored)
+        block = column / kBlock8;
+        row = w.lane % 8;
+        oct = 2 * (w.quarter % 2) + w.lane / 32;
         codes = p.x;
         scales = p.x_scales;
     }
-    // rows first .. first + 7, those past `more` of them read the last one again
+    // the stage from row m0 on; `end`: the slice's, its last row is read again for those behind it
     template <bool WHOLE>
-    __device__ __forceinline__ void load(int64_t first, int more) {
-        const uint8_t *c = codes + first * pitch, *e = scales + first * blocks;
+    __device__ __forceinline__ void load(const Place &w, int64_t m0, int64_t end) {
+        if (WHOLE) {
+            const int64_t first = m0 + 16 * (w.quarter % 2);
+            const uint8_t *c = codes + first * pitch;
+            const uint32_t half = (uint32_t)(w.lane / 32) * 8;
+            exponent = scalar(scales + first * blocks)[(half + row) * (uint32_t)blocks + block];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            code[r] = *reinterpret_cast<const uint32_t *>(scalar(c) + column);
-            exponent[r] = scalar(e)[block];
-            if (WHOLE || r < more) c += pitch, e += blocks;
+            for (int r = 0; r < 8; ++r, c += pitch)
+                code[r] = *reinterpret_cast<const uint2 *>(scalar(c) + (half * (uint32_t)pitch + column));
+        } else {
+            const int64_t first = m0 + 8 * oct;
+            exponent = scales[(first + row < end ? first + row : end - 1) * blocks + block];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                code[r] = *reinterpret_cast<const uint2 *>(codes + (first + r < end ? first + r : end - 1) * pitch + column);
         }
     }
-    __device__ __forceinline__ void clear(int r) { code[r] = 0; }
-    __device__ __forceinline__ uint2 as_bf16(int r) const {
-        const float power = __uint_as_float((uint32_t)exponent[r] << 23);
-        return uint2{word(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[r], power, false)),
-                     word(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[r], power, true))};
+    __device__ __forceinline__ void keep(int r, bool inside) { if (!inside) code[r] = uint2{0, 0}; }
+    template <int R>
+    __device__ __forceinline__ void convert(uint2 (&v)[8], int power, int half) const {
+        // lane R of each sixteen lanes to all of them (they lie in one block of 128 columns)
+        const float mine = __int_as_float(__builtin_amdgcn_update_dpp(0, power, 0x150 + R, 0xf, 0xf, false));
+        const uint32_t c = half ? code[R].y : code[R].x;
+        v[R] = uint2{word(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, mine, false)),
+                     word(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, mine, true))};
+        if constexpr (R < 7) convert<R + 1>(v, power, half);
     }
-    __device__ __forceinline__ f32x4 values(int) const { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+    // columns 4 half .. 4 half + 3
+    __device__ __forceinline__ void as_bf16(uint2 (&v)[8], int half) const { convert<0>(v, exponent << 23, half); }
+    __device__ __forceinline__ f32x4 values(int, int) const { return f32x4{0.f, 0.f, 0.f, 0.f}; }
 };
-template <typename G, bool VEC>
+
+// COLS 8 (bf16 only) or 4 neighbouring columns a load; 1: four, each by itself
+template <typename G, int COLS>
 struct GRun {
     static constexpr bool kIsX = false;
-    typedef typename std::conditional<sizeof(G) == 4, f32x4, uint2>::type Raw;
+    static constexpr int kCols = COLS == 8 ? 8 : 4;
+    typedef typename std::conditional<sizeof(G) == 4 || COLS == 8, u32x4, uint2>::type Raw;
     Raw v[8];
     const G *g;
     int64_t stride;
-    uint32_t column[VEC ? 1 : 4];
+    uint32_t column[COLS == 1 ? 4 : 1];
+    int oct;
 
-    __device__ __forceinline__ GRun(const WgradArgs &p, int64_t, int64_t n0, int quad) {
+    __device__ __forceinline__ GRun(const WgradArgs &p, const Place &w) {
         g = static_cast<const G *>(p.g);
         stride = p.g_stride;
-        const int64_t c = n0 + 4 * quad;
-        if (VEC) {
-            column[0] = (uint32_t)(c < p.n ? c : p.n - 4);
+        const int64_t c = w.n0 + (COLS == 8 ? 8 * (w.lane % 32) : 4 * w.lane);
+        oct = COLS == 8 ? 2 * (w.quarter % 2) + w.lane / 32 : w.quarter;
+        if (COLS > 1) {
+            column[0] = (uint32_t)(c < p.n ? c : p.n - COLS);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) column[VEC ? 0 : j] = (uint32_t)(c + j < p.n ? c + j : p.n - 1);
+            for (int j = 0; j < 4; ++j) column[COLS == 1 ? j : 0] = (uint32_t)(c + j < p.n ? c + j : p.n - 1);
+        }
+    }
+    __device__ __forceinline__ Raw values_at(const G *row, uint32_t half) const {
+        if constexpr (COLS > 1) {
+            return *reinterpret_cast<const Raw *>(row + (half + column[0]));
+        } else if constexpr (sizeof(G) == 4) {
+            return u32x4{__float_as_uint(row[column[0]]), __float_as_uint(row[column[1]]), __float_as_uint(row[column[2]]),
+                         __float_as_uint(row[column[3]])};
+        } else {
+            return uint2{row[column[0]].bits | (uint32_t)row[column[1]].bits << 16,
+                         row[column[2]].bits | (uint32_t)row[column[3]].bits << 16};
         }
     }
     template <bool WHOLE>
-    __device__ __forceinline__ void load(int64_t first, int more) {
-        const G *at = g + first * stride;
+    __device__ __forceinline__ void load(const Place &w, int64_t m0, int64_t end) {
+        if (WHOLE) {
+            const G *at = g + (m0 + (COLS == 8 ? 16 * (w.quarter % 2) : 8 * w.quarter)) * stride;
+            const uint32_t half = COLS == 8 ? (uint32_t)(w.lane / 32) * 8 * (uint32_t)stride : 0;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const G *row = scalar(at);
-            if constexpr (VEC) {
-                v[r] = *reinterpret_cast<const Raw *>(row + column[0]);
-            } else if constexpr (sizeof(G) == 4) {
+            for (int r = 0; r < 8; ++r, at += stride) v[r] = values_at(scalar(at), half);
+        } else {
+            const int64_t first = m0 + 8 * oct;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[r][j] = row[column[j]];
-            } else {
-                v[r] = uint2{row[column[0]].bits | (uint32_t)row[column[1]].bits << 16,
-                             row[column[2]].bits | (uint32_t)row[column[3]].bits << 16};
-            }
-            if (WHOLE || r < more) at += stride;
+            for (int r = 0; r < 8; ++r) v[r] = values_at(g + (first + r < end ? first + r : end - 1) * stride, 0);
         }
     }
-    __device__ __forceinline__ void clear(int r) { v[r] = Raw{}; }
-    __device__ __forceinline__ uint2 as_bf16(int r) const {
-        if constexpr (sizeof(G) == 4) return uint2{bf16_pair(v[r].x, v[r].y), bf16_pair(v[r].z, v[r].w)};
-        else return v[r];
+    __device__ __forceinline__ void keep(int r, bool inside) { if (!inside) v[r] = Raw{}; }
+    __device__ __forceinline__ uint2 pair(int r, int half) const {   // bf16 g
+        if constexpr (COLS == 8) return half ? uint2{v[r].z, v[r].w} : uint2{v[r].x, v[r].y};
+        else return uint2{v[r].x, v[r].y};
     }
-    __device__ __forceinline__ f32x4 values(int r) const {
-        if constexpr (sizeof(G) == 4) return v[r];
-        else return f32x4{__uint_as_float(v[r].x << 16), __uint_as_float(v[r].x & 0xffff0000u),
-                          __uint_as_float(v[r].y << 16), __uint_as_float(v[r].y & 0xffff0000u)};
+    __device__ __forceinline__ void as_bf16(uint2 (&to)[8], int half) const {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            if constexpr (sizeof(G) == 4) {
+                const f32x4 f = values(r, 0);
+                to[r] = uint2{bf16_pair(f.x, f.y), bf16_pair(f.z, f.w)};
+            } else {
+                to[r] = pair(r, half);
+            }
+        }
+    }
+    __device__ __forceinline__ f32x4 values(int r, int half) const {
+        if constexpr (sizeof(G) == 4) {
+            return f32x4{__uint_as_float(v[r].x), __uint_as_float(v[r].y), __uint_as_float(v[r].z), __uint_as_float(v[r].w)};
+        } else {
+            const uint2 p = pair(r, half);
+            return f32x4{__uint_as_float(p.x << 16), __uint_as_float(p.x & 0xffff0000u), __uint_as_float(p.y << 16),
+                         __uint_as_float(p.y & 0xffff0000u)};
+        }
     }
 };
 
-struct Place {                 // of a block and a wave in the result and in the rows
-    int64_t k0, n0, begin, end;
-    int wk, wn, oct, lane;
-    bool live, sums;           // the wave's part of the result lies inside the matrix; it adds up g's columns
-};
+// the largest of 32 neighbouring lanes' words, in all of them
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    auto turned = [&](auto by) {   // by lanes inside sixteen
+        const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + decltype(by)::value, 0xf, 0xf, false);
+        v = other > v ? other : v;
+    };
+    turned(std::integral_constant<int, 1>());
+    turned(std::integral_constant<int, 2>());
+    turned(std::integral_constant<int, 4>());
+    turned(std::integral_constant<int, 8>());
+    const auto pair = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return pair[0] > pair[1] ? pair[0] : pair[1];
+}
+
+// g's rows in the 8-bit format, from the registers on their way to LDS: the input gradient's product wants them, and a pass
+// over g for itself took 65 us (300007 rows of 172, fp32).  A block of 128 columns lies in 32 neighbouring lanes.
+template <typename Run>
+__device__ __forceinline__ void hand_on_rows(const WgradArgs &p, const Place &w, const Run &run, int64_t m0) {
+    const int64_t c = w.n0 + 4 * w.lane, first = m0 + 8 * run.oct;
+    const int64_t blocks = (p.n + kBlock8 - 1) / kBlock8;
+    const bool there = c < blocks * kBlock8;
+    uint8_t *to = p.g_codes + first * blocks * kBlock8 + c;
+    int exponent = 0;                        // of row lane % 8
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        f32x4 f = run.values(r, 0);
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (c + j >= p.n) f[j] = 0.0f;   // (loads there were of other columns)
+            const uint32_t a = __float_as_uint(f[j]) & 0x7fffffffu;
+            top = a > top ? a : top;
+        }
+        const bool finite = !__any((int)(top >= 0x7f800000u));
+        if (!finite) top = __float_as_uint(finite_magnitude(f));
+        const int e = block_exponent(__uint_as_float(lanes_max(top)));
+        if (w.lane % 8 == r) exponent = e;
+        const float inv = pow2(-e);
+        uint32_t code;
+        if (finite) {
+            const f32x4 v = f * inv;
+            code = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v.x, v.y, 0, false);
+            code = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v.z, v.w, (int)code, true);
+        } else {
+            code = encode4(f, inv);
+        }
+        if (there && first + r < w.end) *reinterpret_cast<uint32_t *>(to) = code;
+        to += blocks * kBlock8;
+    }
+    const int r = w.lane % 32;               // the block's first eight lanes store a row's scale each
+    if (r < 8 && there && first + r < w.end) p.g_scales[(first + r) * blocks + c / kBlock8] = (uint8_t)(exponent + 127);
+}
 
 typedef f32x16 Tiles[4][2];
 
-template <typename Run, int SETS>
-__device__ __forceinline__ void wgrad_loop(const WgradArgs &p, const Place &w, uint8_t (&lds)[2][2][kHalfStage], Tiles &acc,
-                                           f32x4 &column_sum) {
-    const Run empty(p, w.k0, w.n0, w.lane);
-    Run raw[2] = {empty, empty};  // (the second unused with one set)
+struct Fragments {             // of one 16-row step: a wave's 128 x 64 of the result
+    bf16x8_t x[4], g[2];
+};
+
+template <typename Run>
+__device__ __forceinline__ void wgrad_loop(const WgradArgs &p, const Place &w, uint8_t *lds, Tiles &acc,
+                                           f32x4 (&column_sum)[2]) {
+    constexpr int kTurns = Run::kCols / 4;   // a wave brings every stage, or every second one
+    Run run(p, w);
+    Fragments frag[2];
     const int idx = w.lane % 32, half = w.lane / 32;
-    auto fetch = [&](auto set, int64_t m0) {
-        Run &run = raw[decltype(set)::value % SETS];
-        const int64_t left = w.end - 1 - (m0 + 8 * w.oct);   // rows behind the first
-        if (left >= 7) run.template load<true>(m0 + 8 * w.oct, 7);
-        else run.template load<false>(left >= 0 ? m0 + 8 * w.oct : w.end - 1, left < 0 ? 0 : (int)left);
+    // of a SIMD's two waves, one that brings x and one that brings g, one brings the even stages and one the odd
+    const int turn = Run::kIsX ? w.quarter / 2 : 1 - w.quarter / 2;
+    auto fetch = [&](int64_t m0) {
+        if (m0 + kRows <= w.end) run.template load<true>(w, m0, w.end);
+        else run.template load<false>(w, m0, w.end);
     };
-    auto stage = [&](auto set, int64_t m0) {
-        Run &run = raw[decltype(set)::value % SETS];
-        const int64_t left = w.end - m0 - 8 * w.oct;  // how many of the eight rows are the slice's
-        if (left < 8) {
+    auto stage = [&](int64_t m0, uint8_t *to) {
+        if (m0 + kRows > w.end) {
+            const int64_t left = w.end - m0 - 8 * run.oct;  // how many of the eight rows are the slice's
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (r >= left) run.clear(r);
+            for (int r = 0; r < 8; ++r) run.keep(r, r < left);
         }
-        uint2 v[8];
+        if constexpr (!Run::kIsX && Run::kCols == 4) {
+            if (w.rows) hand_on_rows(p, w, run, m0);
+        }
 #pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] = run.as_bf16(r);
-        write_columns(lds[decltype(set)::value][Run::kIsX ? 0 : 1], 4 * w.lane, w.oct, v);
-        if (!Run::kIsX && w.sums) {
+        for (int h = 0; h < kTurns; ++h) {
+            uint2 v[8];
+            run.as_bf16(v, h);
+            const int c = kTurns == 2 ? 8 * idx : 4 * w.lane;
+            write_columns(to + (Run::kIsX ? 0 : kHalfStage), c + 4 * h, run.oct, v);
+            if (!Run::kIsX && w.sums) {
 #pragma unroll
-            for (int r = 0; r < 8; ++r) column_sum += run.values(r);
+                for (int r = 0; r < 8; ++r) column_sum[h] += run.values(r, h);
+            }
         }
     };
-    auto multiply = [&](auto set) {
-        if (!w.live) return;
-        const uint8_t *xt = lds[decltype(set)::value][0], *gt = lds[decltype(set)::value][1];
-        // both 16-row steps' fragments are asked for before the first is multiplied
-        bf16x8_t fx[kRows / 16][4], fg[kRows / 16][2];
+    auto bring = [&](int parity, int64_t m0, uint8_t *to) {   // stage m0 to LDS, the wave's next one from memory
+        if (kTurns == 2 && turn != parity) return;
+        stage(m0, to);
+        fetch(m0 + kTurns * kRows);
+    };
+    auto read = [&](auto step, const uint8_t *from) {
+        constexpr int s = decltype(step)::value;
 #pragma unroll
-        for (int s = 0; s < kRows / 16; ++s) {
+        for (int j = 0; j < 2; ++j)
+            frag[s].g[j] =
+                *reinterpret_cast<const bf16x8_t *>(from + kHalfStage + staged(64 * w.wn + 32 * j + idx, 2 * s + half));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            frag[s].x[i] = *reinterpret_cast<const bf16x8_t *>(from + staged(128 * w.wk + 32 * i + idx, 2 * s + half));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&](auto step) {
+        constexpr int s = decltype(step)::value;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                fg[s][j] = *reinterpret_cast<const bf16x8_t *>(gt + staged(64 * w.wn + 32 * j + idx, 2 * s + half));
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                fx[s][i] = *reinterpret_cast<const bf16x8_t *>(xt + staged(128 * w.wk + 32 * i + idx, 2 * s + half));
-        }
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag[s].x[i], frag[s].g[j], acc[i][j], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int s = 0; s < kRows / 16; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fx[s][i], fg[s][j], acc[i][j], 0, 0, 0);
-    };
-    // Stage s lies in LDS buffer s % 2, s + 1 (and with two sets of registers s + 2) in registers or on its way there; as
-    // s + 1 goes into the other buffer, the stage that takes its registers is asked for.  A SIMD has one wave that brings x
-    // and one that brings g: the second does that first and multiplies s behind it, so that its conversions and addresses
-    // run beside the first one's matrix instructions, and the other way round.
-    auto step = [&](auto set, auto other, int64_t m0) {
-        lds_barrier();
-        if (Run::kIsX) multiply(set);
-        stage(other, m0 + kRows);
-        fetch(other, m0 + (1 + SETS) * kRows);
-        if (!Run::kIsX) multiply(set);
     };
     const std::integral_constant<int, 0> even;
     const std::integral_constant<int, 1> odd;
+    // Stage s lies in LDS buffer s % 3, s + 1 in the next one, its first fragments asked for before the barrier that ends s:
+    // no wave waits for LDS behind a barrier.  s + 2 is written meanwhile, from registers, and the stage that takes these
+    // asked for.  The waves that bring g do that first and multiply behind it, so that their conversions and addresses run
+    // beside the others' matrix instructions, and the other way round.
+    uint8_t *now = lds, *next = lds + 2 * kHalfStage;
+    auto step = [&](int parity, int64_t m0) {
+        if (!Run::kIsX) bring(1 - parity, m0 + kRows, next);
+        if (w.live) {
+            read(even, now);
+            read(odd, now);
+            multiply(even);
+            multiply(odd);
+        }
+        if (Run::kIsX) bring(1 - parity, m0 + kRows, next);
+        lds_barrier();
+        uint8_t *const was = now;
+        now = next, next = was;
+    };
     if (w.begin >= w.end) return;
-    fetch(even, w.begin);
-    if (SETS == 2) fetch(odd, w.begin + kRows);
-    stage(even, w.begin);
-    fetch(even, w.begin + SETS * kRows);
+    if (kTurns == 2) {
+        fetch(w.begin + turn * kRows);
+        if (turn == 0) bring(0, w.begin, now);
+    } else {
+        fetch(w.begin);
+        bring(0, w.begin, now);
+    }
+    lds_barrier();
     for (int64_t m0 = w.begin; m0 < w.end; m0 += 2 * kRows) {  // (a stage past the end holds zeros)
-        step(even, odd, m0);
-        step(odd, even, m0 + kRows);
+        step(0, m0);
+        step(1, m0 + kRows);
     }
 }
 
-template <typename G, bool VEC>
+template <typename G, int COLS>
 __global__ __launch_bounds__(512, 2) void fp8_wgrad_kernel(const WgradArgs p) {
-    __shared__ __align__(16) uint8_t lds[2][2][kHalfStage];   // stage parity; x, g
+    __shared__ __align__(16) uint8_t lds[2 * 2 * kHalfStage];   // stages; x, g
     const int lane = (int)threadIdx.x % 64;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
     const int kt = (int)blockIdx.x / p.tiles_n, nt = (int)blockIdx.x % p.tiles_n;
     const int64_t slice = blockIdx.y;
     Place w;
-    w.wk = wave / 4, w.wn = wave % 4, w.oct = wave % 4, w.lane = lane;
+    w.wk = wave / 4, w.wn = wave % 4, w.quarter = wave % 4, w.lane = lane;
     w.k0 = (int64_t)kt * kTile, w.n0 = (int64_t)nt * kTile;
     w.begin = slice * p.rows_per_slice;
     w.end = w.begin + p.rows_per_slice < p.rows ? w.begin + p.rows_per_slice : p.rows;
     w.live = w.k0 + 128 * w.wk < p.k && w.n0 + 64 * w.wn < p.n;
     w.sums = kt == 0 && p.bias_out;
+    w.rows = kt == 0 && p.g_codes;
     const int idx = lane % 32, half = lane / 32;
 
     Tiles acc;
@@ -266,12 +392,13 @@ __global__ __launch_bounds__(512, 2) void fp8_wgrad_kernel(const WgradArgs p) {
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    f32x4 column_sum = {0.f, 0.f, 0.f, 0.f};
+    f32x4 column_sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 
     // Waves 0-3 bring x, 4-7 bring g: the whole loop apart, with the same barriers, so that neither's registers are merged
     // with the other's (which would wait for the loads in flight).
-    if (wave < 4) wgrad_loop<XRun, 2>(p, w, lds, acc, column_sum);
-    else wgrad_loop<GRun<G, VEC>, sizeof(G) == 2 ? 2 : 1>(p, w, lds, acc, column_sum);  // (two sets of fp32 g would spill)
+    typedef GRun<G, COLS> Gradient;
+    if (wave < 4) wgrad_loop<XRun>(p, w, lds, acc, column_sum);
+    else wgrad_loop<Gradient>(p, w, lds, acc, column_sum);
 
     // register r of lane l holds row (r % 4) + 8 (r / 4) + 4 (l / 32), column l % 32 of its 32 x 32 tile
     float *out = p.out + slice * p.k * p.n;
@@ -286,16 +413,22 @@ __global__ __launch_bounds__(512, 2) void fp8_wgrad_kernel(const WgradArgs p) {
                 if (k < p.k && n < p.n) out[k * p.n + n] = acc[i][j][r];
             }
         }
-    if (w.sums) {
-        f32x4 *parts = reinterpret_cast<f32x4 *>(lds);
+    if (w.sums) {   // each wave's (with eight columns a thread, each half-wave's) sums of its rows, then all rows'
+        constexpr int kParts = Gradient::kCols == 8 ? 8 : 4;
+        float *parts = reinterpret_cast<float *>(lds);   // [kParts][kTile]
         const int tid = (int)threadIdx.x;
         __syncthreads();
-        if (wave >= 4) parts[tid - 256] = column_sum;
+        if (wave >= 4) {
+            const int part = Gradient::kCols == 8 ? 2 * w.quarter + half : w.quarter;
+            f32x4 *at = reinterpret_cast<f32x4 *>(parts + part * kTile + (Gradient::kCols == 8 ? 8 * idx : 4 * lane));
+            at[0] = column_sum[0];
+            if (Gradient::kCols == 8) at[1] = column_sum[1];
+        }
         __syncthreads();
-        if (tid < 64) {
-            f32x4 total = parts[tid];
-            for (int q = 1; q < 4; ++q) total += parts[tid + 64 * q];
-            store4<false>(p.bias_out + slice * p.n, (int64_t)(w.n0 + 4 * tid), p.n, total);
+        if (tid < kTile && w.n0 + tid < p.n) {
+            float total = parts[tid];
+            for (int q = 1; q < kParts; ++q) total += parts[tid + q * kTile];
+            p.bias_out[slice * p.n + w.n0 + tid] = total;
         }
     }
 }
@@ -332,6 +465,15 @@ extern "C" int64_t gnnagg_fp8_weight_gradient_workspace_bytes(int64_t rows, int6
 extern "C" int gnnagg_fp8_weight_gradient(const uint8_t *x, const uint8_t *x_scales, const void *g, int64_t g_stride,
                                           int g_dtype, float *grad_w, float *grad_bias, void *workspace,
                                           int64_t workspace_bytes, int64_t rows, int64_t k, int64_t n, void *stream) {
+    return gnnagg_fp8_weight_gradient_and_rows(x, x_scales, g, g_stride, g_dtype, grad_w, grad_bias, nullptr, nullptr,
+                                               workspace, workspace_bytes, rows, k, n, stream);
+}
+
+extern "C" int gnnagg_fp8_weight_gradient_and_rows(const uint8_t *x, const uint8_t *x_scales, const void *g,
+                                                   int64_t g_stride, int g_dtype, float *grad_w, float *grad_bias,
+                                                   uint8_t *g_codes, uint8_t *g_scales, void *workspace,
+                                                   int64_t workspace_bytes, int64_t rows, int64_t k, int64_t n,
+                                                   void *stream) {
     GNNAGG_REQUIRE(rows >= 0 && k >= 0 && n >= 0, "negative size");
     GNNAGG_REQUIRE(known_dtype(g_dtype), "unknown dtype");
     if (k == 0 || n == 0) return GNNAGG_OK;
@@ -339,6 +481,8 @@ extern "C" int gnnagg_fp8_weight_gradient(const uint8_t *x, const uint8_t *x_sca
     GNNAGG_REQUIRE(grad_w && (rows == 0 || (x && x_scales && g)), "null x/scales/g/grad_w");
     GNNAGG_REQUIRE(g_stride >= n, "a row stride is below the width");
     GNNAGG_REQUIRE(reinterpret_cast<uintptr_t>(x) % 4 == 0, "codes must be 4-byte aligned");
+    GNNAGG_REQUIRE((g_codes != nullptr) == (g_scales != nullptr), "codes of g without scales, or the other way round");
+    GNNAGG_REQUIRE(reinterpret_cast<uintptr_t>(g_codes) % 4 == 0, "codes of g must be 4-byte aligned");
     const int64_t slices = wgrad_slices(rows, k, n), need = gnnagg_fp8_weight_gradient_workspace_bytes(rows, k, n);
     GNNAGG_REQUIRE(workspace_bytes >= need && (need == 0 || workspace) && reinterpret_cast<uintptr_t>(workspace) % 4 == 0,
                    "workspace of %lld bytes is too small, null or misaligned", (long long)workspace_bytes);
@@ -346,21 +490,34 @@ extern "C" int gnnagg_fp8_weight_gradient(const uint8_t *x, const uint8_t *x_sca
     float *bias_parts = !grad_bias ? nullptr : slices == 1 ? grad_bias : parts + slices * k * n;
     const int64_t per = (rows + slices - 1) / slices;
     const int64_t tiles_k = (k + kTile - 1) / kTile, tiles_n = (n + kTile - 1) / kTile;
-    WgradArgs p{x, x_scales, g, parts, bias_parts, g_stride, rows, (per + kRows - 1) / kRows * kRows, k, n,
+    // With one tile along k the pass is bound by memory and the rows' conversion runs beside its loads; with more, the first
+    // tile's blocks alone would convert and the rest wait for them.
+    const bool rows_here = tiles_k == 1;
+    if (g_codes && !rows_here)
+        if (const int rc = gnnagg_fp8_quantize_rows(g, g_stride, g_codes, g_scales, rows, n, g_dtype, stream)) return rc;
+    WgradArgs p{x, x_scales, g, parts, bias_parts, rows_here ? g_codes : nullptr, g_scales, g_stride, rows, (per + kRows - 1) / kRows * kRows, k, n,
                 (int)(pad128(k) / kBlock8), (int)tiles_n};
     if (tiles_k * tiles_n > 0x7fffffff) return fail(GNNAGG_ERR_UNSUPPORTED, "too many tiles");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)(tiles_k * tiles_n), (unsigned)slices);
-    auto go = [&](auto type, auto v) {
-        hipLaunchKernelGGL((fp8_wgrad_kernel<decltype(type), decltype(v)::value>), grid, dim3(512), 0, st, p);
+    auto go = [&](auto type, auto cols) {
+        hipLaunchKernelGGL((fp8_wgrad_kernel<decltype(type), decltype(cols)::value>), grid, dim3(512), 0, st, p);
     };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 4> four;
+    const std::integral_constant<int, 8> eight;
     const bool vec = vec4_rows(g, g_stride, n, g_dtype);
+    // (sixteen bytes of bf16 a load where rows allow it and offsets of eight rows fit 32 bits;
+    // where rows are handed on that takes too many registers)
+    const bool wide = g_dtype == GNNAGG_BF16 && !p.g_codes && n % 8 == 0 && g_stride % 8 == 0 && g_stride < (int64_t(1) << 27) &&
+                      reinterpret_cast<uintptr_t>(g) % 16 == 0;
     if (g_dtype == GNNAGG_F32) {
-        if (vec) go(float(), std::true_type());
-        else go(float(), std::false_type());
+        if (vec) go(float(), four);
+        else go(float(), one);
     } else {
-        if (vec) go(bf16_t(), std::true_type());
-        else go(bf16_t(), std::false_type());
+        if (wide) go(bf16_t(), eight);
+        else if (vec) go(bf16_t(), four);
+        else go(bf16_t(), one);
     }
     GNNAGG_HIP(hipGetLastError());
     if (slices == 1) return GNNAGG_OK;

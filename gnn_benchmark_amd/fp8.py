@@ -157,6 +157,12 @@ def _product(x, weight, bias, out_dtype, input_gradient=False):
 
 def weight_gradient(x: QuantizedRows, g: torch.Tensor, with_bias: bool = False):
     """``x^T @ bf16(g)``, fp32 [x.cols, n]; with ``with_bias`` the pair of it and ``g``'s column sums (fp32)."""
+    grad_w, grad_b, _ = _weight_gradient(x, g, with_bias, False)
+    return (grad_w, grad_b) if with_bias else grad_w
+
+
+def _weight_gradient(x: QuantizedRows, g: torch.Tensor, with_bias: bool, with_rows: bool):
+    """(weight gradient, column sums or None, g in the 8-bit format or None)"""
     x.check("x")
     check_gpu(g, "g", x.codes.device)
     code = dtype_code(g.dtype, "g")
@@ -168,26 +174,27 @@ def weight_gradient(x: QuantizedRows, g: torch.Tensor, with_bias: bool = False):
     nbytes = int(L.gnnagg_fp8_weight_gradient_workspace_bytes(rows, k, n))
     grad_w = torch.empty(k, n, dtype=torch.float32, device=device)
     grad_b = torch.empty(n, dtype=torch.float32, device=device) if with_bias else None
+    g_rows = QuantizedRows.empty(rows, n, device) if with_rows else None
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     with _lib.on_device(device):
-        _lib.check(L.gnnagg_fp8_weight_gradient(
+        _lib.check(L.gnnagg_fp8_weight_gradient_and_rows(
             address(x.codes), address(x.scales), address(g), row_stride(g), code, address(grad_w), address(grad_b),
+            address(g_rows.codes) if with_rows else None, address(g_rows.scales) if with_rows else None,
             address(workspace), nbytes, rows, k, n, _lib.raw_stream(device)))
-    return (grad_w, grad_b) if with_bias else grad_w
+    return grad_w, grad_b, g_rows
 
 
 def _product_gradients(rows: QuantizedRows, weight: QuantizedWeight, g: torch.Tensor, want_x: bool, want_w: bool,
                        want_b: bool, x_dtype, w_dtype, b_dtype):
     """(grad of the rows, of the weight, of the bias) of ``rows @ weight + bias``, each None where it is not wanted."""
-    grad_x = grad_w = grad_b = None
+    grad_x = grad_w = grad_b = g_rows = None
     g = as_rows(g)
+    if want_w or want_b:  # (the bias's sums come with the weight gradient's pass, beside a frozen weight too)
+        grad_w, grad_b, g_rows = _weight_gradient(rows, g, want_b, want_x)
+        grad_w = grad_w.to(w_dtype) if want_w else None
+        grad_b = grad_b.to(b_dtype) if want_b else None
     if want_x:
-        grad_x = _product(_quantize_rows(g), weight, None, x_dtype, input_gradient=True)
-    if want_b:  # (beside a frozen weight too: the sums come with the weight gradient's pass)
-        grad_w, grad_b = weight_gradient(rows, g, True)
-        grad_w, grad_b = grad_w.to(w_dtype) if want_w else None, grad_b.to(b_dtype)
-    elif want_w:
-        grad_w = weight_gradient(rows, g).to(w_dtype)
+        grad_x = _product(g_rows or _quantize_rows(g), weight, None, x_dtype, input_gradient=True)
     return grad_x, grad_w, grad_b
 
 
