@@ -315,32 +315,6 @@ def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
-class _NoGuard:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NO_GUARD = _NoGuard()
-
-
-def on_device(device):
-    """``with`` block on a tensor's device: nothing to do where it is the current one, which is most of the time (the
-    general guard costs more than a small kernel's launch)."""
-    import torch
-
-    return _NO_GUARD if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
-
-
-def raw_stream(device) -> int:
-    """Handle of the device's current stream, without an object around it."""
-    import torch
-
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
 _CHECKED_INDEX = {}
 
 

@@ -1,10 +1,11 @@
-// The pybind11 module `train_ops`: the calls of the training operators that a single token or a small model makes --
-// RMS norm, rows into the 8-bit format, the 8-bit product, the AdamW step -- from checked arguments to the C entry point
-// on the current stream.  Their kernels take 4 to 10 us there, which the same checks, allocations and foreign calls
-// written in Python took several times over (one row of 4096: norm with 8-bit output 16.5 us a call from Python,
-// product 11 us, the step of ten small tensors 26 us).  `norm.py`, `fp8.py` and `optim.py` call it; it holds nothing from
-// one call to the next.
+// The pybind11 module `train_ops`: the calls of the training operators -- RMS norm, the 8-bit format and its products with
+// their gradients, the AdamW step -- from checked arguments to the C entry points on the current stream.  On a single token
+// or a small model their kernels take 4 to 10 us, which the same checks, allocations and foreign calls written in Python
+// took several times over (one row of 4096: norm with 8-bit output 16.5 us a call from Python, product 11 us, the step of
+// ten small tensors 26 us).  `norm.py`, `fp8.py` and `optim.py` call it; it holds nothing from one call to the next.
 #include <torch/extension.h>
+
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -32,6 +33,8 @@ PyObject *error_class = nullptr;  // the package's GnnAggError
 
 void check_rc(int rc) {
     if (rc == GNNAGG_OK) return;
+    // (a backward pass runs on the engine's threads, which do not hold the interpreter)
+    TORCH_CHECK(PyGILState_Check(), "libgnnagg error ", rc, ": ", gnnagg_last_error());
     py::object error = py::reinterpret_steal<py::object>(PyObject_CallFunction(error_class, "is", rc, gnnagg_last_error()));
     if (error) PyErr_SetObject(error_class, error.ptr());
     throw py::error_already_set();
@@ -265,6 +268,258 @@ std::tuple<Tensor, Tensor, OptTensor> public_rms_norm_fp8(const Tensor &x, const
     return rms_norm_fp8(x, weight, eps, residual, relu);
 }
 
+// (codes by output, codes by input, scales), either codes where asked for; a weight stored by output is read where it lies
+std::tuple<OptTensor, OptTensor, Tensor> quantize_weight(const Tensor &w_, bool by_output, bool by_input) {
+    check_gpu(w_, "the weight");
+    const int code = dtype_code(w_.scalar_type(), "the weight");
+    TORCH_CHECK(w_.dim() == 2 && w_.numel() > 0, "Input mismatch: the weight must be [k, n], neither zero");
+    const int64_t k = w_.size(0), n = w_.size(1);
+    if (w_.stride(1) != 1 && w_.stride(0) == 1 && w_.stride(1) >= k) {  // its transpose with the roles exchanged
+        auto [codes, codes_by_input, scales] = quantize_weight(w_.t(), by_input, by_output);
+        return {codes_by_input, codes, scales.t()};
+    }
+    const Rows w(w_);
+    OptTensor codes, codes_by_input;
+    const auto type = w_.options().dtype(at::kFloat8_e4m3fn);
+    if (by_output) codes = at::empty({n, padded(k)}, type);
+    if (by_input) codes_by_input = at::empty({k, padded(n)}, type);
+    const Tensor scales = at::empty({padded(k) / kBlock, padded(n) / kBlock}, type.dtype(at::kFloat8_e8m0fnu));
+    const Place place(w_);
+    check_rc(gnnagg_fp8_quantize_weight(w.data, w.stride, codes ? bytes(*codes) : nullptr,
+                                        codes_by_input ? bytes(*codes_by_input) : nullptr, bytes(scales), k, n, code,
+                                        place.stream));
+    return {codes, codes_by_input, scales};
+}
+
+std::tuple<OptTensor, OptTensor, Tensor> public_quantize_weight(const Tensor &w, bool by_input) {
+    if (at::GradMode::is_enabled()) refuse_grad(w);
+    return quantize_weight(w, true, by_input);
+}
+
+// (x^T bf16(g), g's column sums or None, codes and scales of g's rows or None)
+std::tuple<Tensor, OptTensor, OptTensor, OptTensor> weight_gradient(const Tensor &x, const Tensor &x_scales, int64_t k,
+                                                                    const Tensor &g_, bool with_bias, bool with_rows) {
+    check_rows(x, x_scales, k);
+    check_gpu(g_, "g", x);
+    const int code = dtype_code(g_.scalar_type(), "g");
+    TORCH_CHECK(g_.dim() == 2 && g_.size(0) == x.size(0) && g_.size(1) > 0, "Input mismatch: g must be [rows of x, outputs]");
+    const Rows g(g_);
+    const int64_t rows = g.rows, n = g.width;
+    const auto type = x.options().dtype(at::kFloat);
+    const int64_t nbytes = gnnagg_fp8_weight_gradient_workspace_bytes(rows, k, n);
+    const Tensor grad_w = at::empty({k, n}, type);
+    OptTensor grad_b, codes, scales;
+    if (with_bias) grad_b = at::empty({n}, type);
+    if (with_rows) {
+        auto [c, e] = empty_rows(rows, n, x);
+        codes = c, scales = e;
+    }
+    Tensor workspace;
+    if (nbytes) workspace = at::empty({nbytes}, type.dtype(at::kByte));
+    const Place place(x);
+    check_rc(gnnagg_fp8_weight_gradient_and_rows(
+        bytes(x), bytes(x_scales), g.data, g.stride, code, grad_w.data_ptr<float>(),
+        grad_b ? grad_b->data_ptr<float>() : nullptr, codes ? bytes(*codes) : nullptr, scales ? bytes(*scales) : nullptr,
+        nbytes ? workspace.data_ptr() : nullptr, nbytes, rows, k, n, place.stream));
+    return {grad_w, grad_b, codes, scales};
+}
+
+// (gradient of x and of the residual, gradient of the weight in its type)
+std::tuple<Tensor, Tensor> rms_norm_backward(const Tensor &grad_y_, const OptTensor &grad_h_, const Tensor &h_,
+                                             const Tensor &weight_, double eps, bool relu) {
+    const Rows grad_y(grad_y_), h(h_);
+    c10::optional<Rows> grad_h;
+    if (grad_h_) grad_h.emplace(*grad_h_);
+    const Tensor weight = weight_.is_contiguous() ? weight_ : weight_.contiguous();
+    const int64_t nbytes = gnnagg_rms_norm_backward_workspace_bytes(h.rows, h.width);
+    const Tensor grad_x = at::empty(h_.sizes(), h_.options()), grad_w = at::empty({h.width}, h_.options().dtype(at::kFloat));
+    const Tensor workspace = at::empty({nbytes}, h_.options().dtype(at::kByte));
+    const Place place(h_);
+    check_rc(gnnagg_rms_norm_backward(grad_y.data, grad_y.stride, grad_h ? grad_h->data : nullptr,
+                                      grad_h ? grad_h->stride : 0, h.data, h.stride, weight.const_data_ptr(),
+                                      dtype_code(weight.scalar_type(), "the norm's weight"), eps, relu, grad_x.data_ptr(),
+                                      h.width, grad_w.data_ptr<float>(), workspace.data_ptr(), nbytes, h.rows, h.width,
+                                      dtype_code(h_.scalar_type(), "x"), place.stream));
+    return {grad_x, grad_w.to(weight_.scalar_type())};
+}
+
+// ---------------------------------------------------------------------------------------------- differentiable forms
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// A gradient's own gradient is refused when it is asked for.
+variable_list once_differentiable(variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    auto refuse = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that is differentiable once", (int64_t)grads.size());
+    for (Tensor &t : grads)
+        if (t.defined()) t = t.detach().set_requires_grad(true);  // (so that there is something to refuse)
+    return (*refuse)(std::move(grads));
+}
+
+OptTensor given(const Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+struct ProductGradients {
+    Tensor x, w, b;
+};
+
+// gradients of rows @ weight + bias, each where it is wanted
+ProductGradients product_gradients(const Tensor &codes, const Tensor &scales, const Tensor &by_input, const Tensor &w_scales,
+                                   int64_t k, const Tensor &g, bool want_x, bool want_w, bool want_b, at::ScalarType x_type,
+                                   at::ScalarType w_type, at::ScalarType b_type) {
+    ProductGradients grads;
+    const int64_t n = g.size(1);
+    OptTensor g_codes, g_scales;
+    if (want_w || want_b) {  // (the bias's sums come with the weight gradient's pass, beside a frozen weight too)
+        auto [w, b, c, e] = weight_gradient(codes, scales, k, g, want_b, want_x);
+        if (want_w) grads.w = w.to(w_type);
+        if (want_b) grads.b = b->to(b_type);
+        g_codes = c, g_scales = e;
+    }
+    if (want_x) {
+        if (!g_codes) {
+            auto [c, e] = quantize_rows(g);
+            g_codes = c, g_scales = e;
+        }
+        grads.x = product(*g_codes, *g_scales, n, by_input, w_scales, k, n, OptTensor(), x_type, OptTensor(), true);
+    }
+    return grads;
+}
+
+void check_linear(const Tensor &x, const Tensor &w, const OptTensor &bias) {
+    check_gpu(x, "x");
+    check_gpu(w, "the weight", x);
+    dtype_code(x.scalar_type(), "x");
+    dtype_code(w.scalar_type(), "the weight");
+    TORCH_CHECK(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(0) && w.numel() > 0, "Input mismatch: x ", x.sizes(),
+                " against a weight ", w.sizes());
+    if (bias) {
+        check_gpu(*bias, "the bias", x);
+        dtype_code(bias->scalar_type(), "the bias");
+        TORCH_CHECK(bias->dim() == 1 && bias->numel() == w.size(1), "Input mismatch: the bias must hold one value per output");
+    }
+}
+
+std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t last) {
+    std::vector<int64_t> shape(sizes.begin(), sizes.end());
+    shape.back() = last;
+    return shape;
+}
+
+Tensor flat(const Tensor &t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
+
+bool wanted(const OptTensor &t) { return at::GradMode::is_enabled() && t && t->requires_grad(); }
+
+struct LinearFunction : torch::autograd::Function<LinearFunction> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &bias, bool for_x) {
+        auto [codes, scales] = quantize_rows(flat(x));
+        auto [w_codes, by_input, w_scales] = quantize_weight(w, true, for_x);
+        const Tensor out = product(codes, scales, w.size(0), w_codes, w_scales, w.size(0), w.size(1), bias, x.scalar_type(),
+                                   OptTensor(), false);
+        ctx->save_for_backward({codes, scales, by_input ? *by_input : Tensor(), w_scales});
+        ctx->saved_data["shape"] = x.sizes().vec();
+        ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)w.scalar_type(),
+                                                        bias ? (int64_t)bias->scalar_type() : -1};
+        return x.dim() == 2 ? out : out.view(with_last(x.sizes(), w.size(1)));
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const auto saved = ctx->get_saved_variables();
+        const auto shape = ctx->saved_data["shape"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
+        const bool has_bias = types[2] >= 0;
+        const auto grads = product_gradients(saved[0], saved[1], saved[2], saved[3], shape.back(), flat(g[0]),
+                                             ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                             has_bias && ctx->needs_input_grad(2), (at::ScalarType)types[0],
+                                             (at::ScalarType)types[1], (at::ScalarType)types[2]);
+        return once_differentiable({grads.x.defined() && shape.size() != 2 ? grads.x.view(shape) : grads.x, grads.w, grads.b,
+                                    Tensor()});
+    }
+};
+
+Tensor linear(const Tensor &x, const Tensor &w, const OptTensor &bias) {
+    check_linear(x, w, bias);
+    return LinearFunction::apply(x, w, bias, wanted(x));
+}
+
+struct RmsNormFunction : torch::autograd::Function<RmsNormFunction> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const OptTensor &residual, const Tensor &weight,
+                                 double eps, bool relu) {
+        auto [y, h] = rms_norm(x, weight, eps, residual, relu, OptTensor());
+        ctx->save_for_backward({h ? *h : x, weight});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["relu"] = relu;
+        ctx->set_materialize_grads(false);
+        return h ? variable_list{y, *h} : variable_list{y};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const auto saved = ctx->get_saved_variables();
+        const bool has_residual = g.size() == 2;
+        Tensor grad_x = has_residual ? g[1] : Tensor(), grad_w;  // (only the residual stream was used)
+        if (g[0].defined())
+            std::tie(grad_x, grad_w) = rms_norm_backward(g[0], given(grad_x), saved[0], saved[1],
+                                                         ctx->saved_data["eps"].toDouble(), ctx->saved_data["relu"].toBool());
+        const bool for_x = ctx->needs_input_grad(0), for_residual = has_residual && ctx->needs_input_grad(1);
+        const bool for_weight = ctx->needs_input_grad(has_residual ? 2 : 1);
+        return once_differentiable({for_x ? grad_x : Tensor(), for_residual ? grad_x : Tensor(),
+                                    for_weight ? grad_w : Tensor(), Tensor(), Tensor()});
+    }
+};
+
+std::tuple<Tensor, Tensor> differentiable_rms_norm(const Tensor &x, const Tensor &weight, double eps, const OptTensor &residual,
+                                                   bool relu) {
+    NormCall::check(x, weight, residual);
+    const auto out = RmsNormFunction::apply(x, residual, weight, eps, relu);
+    return {out[0], residual ? out[1] : x};
+}
+
+struct NormLinearFunction : torch::autograd::Function<NormLinearFunction> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const OptTensor &residual, const Tensor &norm_weight,
+                                 const Tensor &w, const OptTensor &bias, double eps, bool relu, bool for_rows) {
+        auto [codes, scales, h] = rms_norm_fp8(x, norm_weight, eps, residual, relu);
+        auto [w_codes, by_input, w_scales] = quantize_weight(w, true, for_rows);
+        Tensor out = product(codes, scales, w.size(0), w_codes, w_scales, w.size(0), w.size(1), bias, x.scalar_type(),
+                             OptTensor(), false);
+        ctx->save_for_backward({h ? *h : x, norm_weight, codes, scales, by_input ? *by_input : Tensor(), w_scales});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["relu"] = relu;
+        ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)w.scalar_type(),
+                                                        bias ? (int64_t)bias->scalar_type() : -1};
+        ctx->set_materialize_grads(false);
+        if (x.dim() != 2) out = out.view(with_last(x.sizes(), w.size(1)));
+        return h ? variable_list{out, *h} : variable_list{out};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const auto saved = ctx->get_saved_variables();
+        const auto types = ctx->saved_data["types"].toIntVector();
+        const bool has_residual = g.size() == 2, has_bias = types[2] >= 0;
+        const int at = has_residual ? 1 : 0;
+        const bool for_x = ctx->needs_input_grad(0), for_residual = has_residual && ctx->needs_input_grad(1);
+        const bool for_norm = ctx->needs_input_grad(1 + at), for_w = ctx->needs_input_grad(2 + at);
+        const bool for_bias = has_bias && ctx->needs_input_grad(3 + at);
+        ProductGradients grads;
+        Tensor grad_x = has_residual ? g[1] : Tensor(), grad_norm;
+        if (g[0].defined()) {
+            grads = product_gradients(saved[2], saved[3], saved[4], saved[5], saved[0].size(-1), flat(g[0]),
+                                      for_x || for_residual || for_norm, for_w, for_bias, (at::ScalarType)types[0],
+                                      (at::ScalarType)types[1], (at::ScalarType)types[2]);
+            if (grads.x.defined())
+                std::tie(grad_x, grad_norm) = rms_norm_backward(grads.x, given(grad_x), saved[0], saved[1],
+                                                                ctx->saved_data["eps"].toDouble(),
+                                                                ctx->saved_data["relu"].toBool());
+        }
+        return once_differentiable({for_x ? grad_x : Tensor(), for_residual ? grad_x : Tensor(),
+                                    for_norm ? grad_norm : Tensor(), grads.w, grads.b, Tensor(), Tensor(), Tensor()});
+    }
+};
+
+std::tuple<Tensor, Tensor> norm_linear(const Tensor &x, const Tensor &norm_weight, double eps, const Tensor &w,
+                                       const OptTensor &bias, const OptTensor &residual, bool relu) {
+    NormCall::check(x, norm_weight, residual);
+    check_linear(x, w, bias);
+    const auto out = NormLinearFunction::apply(x, residual, norm_weight, w, bias, eps, relu,
+                                               wanted(x) || wanted(residual) || wanted(norm_weight));
+    return {out[0], residual ? out[1] : x};
+}
+
 // ----------------------------------------------------------------------------------------------------------- AdamW
 typedef std::vector<Tensor> Tensors;
 
@@ -391,12 +646,15 @@ PYBIND11_MODULE(train_ops, m) {
                                  ": rebuild both (gnn_benchmark_amd/ext/build.sh)");
     m.doc() = "Calls of the training operators (libgnnagg.so underneath)";
     m.def("set_error_class", [](py::object cls) { error_class = cls.release().ptr(); });
-    m.def("rms_norm", &rms_norm);
-    m.def("rms_norm_fp8_forward", &rms_norm_fp8);   // (inside a differentiable operator's forward)
+    m.def("rms_norm", &differentiable_rms_norm);
+    m.def("rms_norm_forward", &rms_norm);
+    m.def("rms_norm_backward", &rms_norm_backward);
     m.def("rms_norm_fp8", &public_rms_norm_fp8);
-    m.def("quantize_rows_forward", &quantize_rows);
     m.def("quantize_rows", &public_quantize_rows);
-    m.def("product_forward", &product);
+    m.def("quantize_weight", &public_quantize_weight);
     m.def("product", &public_product);
+    m.def("weight_gradient", &weight_gradient);
+    m.def("linear", &linear);
+    m.def("norm_linear", &norm_linear);
     m.def("adamw_step", &adamw_step);
 }

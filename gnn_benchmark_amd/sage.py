@@ -36,7 +36,7 @@ import torch
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
-from . import _lib, aggregator, fp8
+from . import _lib, aggregator, ext, fp8
 from . import norm as rms
 from .gcn import (_FORMS, _mean_nll, input_gradient, plain_product, scored_rows, stacked_product,
                   weight_and_bias_gradient, weight_gradient)
@@ -146,7 +146,7 @@ class _ResidualRmsNormRelu(torch.autograd.Function):
     def forward(ctx, z, residual, weight, eps):
         rows, feat = z.shape
         cat = torch.empty(rows, 2 * feat, dtype=torch.float32, device=z.device)
-        _, h = rms._forward(z, weight, eps, residual, True, y=cat[:, feat:])
+        _, h = ext.train_ops().rms_norm_forward(z, weight, eps, residual, True, cat[:, feat:])
         ctx.save_for_backward(z if h is None else h, weight)
         ctx.eps = eps
         ctx.set_materialize_grads(False)
@@ -158,7 +158,8 @@ class _ResidualRmsNormRelu(torch.autograd.Function):
         h, weight = ctx.saved_tensors
         grad_z, grad_weight = grad_h, None
         if grad_cat is not None:  # of its right half: the left half belongs to nobody
-            grad_z, grad_weight = rms._backward(grad_cat[:, h.size(1):], grad_h, h, weight, ctx.eps, True)
+            grad_z, grad_weight = ext.train_ops().rms_norm_backward(grad_cat[:, h.size(1):], grad_h, h, weight, ctx.eps,
+                                                                       True)
         want = ctx.needs_input_grad
         return (grad_z if want[0] else None, grad_z if want[1] else None, grad_weight if want[2] else None, None)
 

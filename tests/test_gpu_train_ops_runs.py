@@ -161,3 +161,37 @@ def test_the_weight_gradients_pass_hands_on_the_rows(m, k, n, dtype):
         off = 2 * (m + 8) * o.HALF32 * g.double().abs().sum(0)
         assert bool(((grad_b.double() - plain_b.double()).abs() <= off)[fine].all())
         assert torch.equal(grad_b.isfinite(), fine) and torch.equal(plain_b.isfinite(), fine)
+
+
+def test_a_gradients_gradient_is_refused():
+    x = torch.randn(40, 96, device="cuda", requires_grad=True)
+    w = torch.randn(96, 33, device="cuda", requires_grad=True)
+    nw = torch.ones(96, device="cuda", requires_grad=True)
+    for out in (fp8.linear(x, w), norm.rms_norm(x, nw)[0], fp8.norm_linear(x, nw, 1e-6, w, residual=x)[0]):
+        (once,) = torch.autograd.grad((out.sum(),), (x,), create_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            (once.sum() + x.sum()).backward()
+
+
+def test_only_what_is_wanted_gets_a_gradient():
+    """Every choice of leaves that want a gradient gives the gradients that all of them together give."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    normal = lambda *shape: torch.randn(*shape, device="cuda", generator=gen)  # noqa: E731
+    values = [normal(50, 200), normal(50, 200), 1 + 0.1 * normal(200), normal(200, 70) / 14, normal(70)]
+    g, gh = normal(50, 70), normal(50, 200)
+
+    def grads(which):
+        leaves = [v.clone().requires_grad_(i in which) for i, v in enumerate(values)]
+        out, h = fp8.norm_linear(leaves[0], leaves[2], 1e-6, leaves[3], leaves[4], residual=leaves[1])
+        used = [leaves[i] for i in which]
+        return torch.autograd.grad((out, h) if {0, 1} & set(which) else (out,), used, (g, gh) if {0, 1} & set(which) else (g,))
+
+    every = grads([0, 1, 2, 3, 4])
+    for which in ([0], [1], [3], [4], [0, 3], [1, 4], [3, 4]):
+        for i, got in zip(which, grads(which)):
+            assert torch.equal(got, every[i]), (which, i)
+    only_norm = grads([2])[0]                               # (h needs no gradient there, so none comes back through it)
+    x = (values[0] + values[1]).requires_grad_()
+    nw = values[2].clone().requires_grad_()
+    out, _ = fp8.norm_linear(x, nw, 1e-6, values[3], values[4])
+    assert torch.equal(only_norm, torch.autograd.grad((out,), (nw,), (g,))[0])
