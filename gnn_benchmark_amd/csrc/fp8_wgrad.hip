@@ -9,12 +9,19 @@
 //
 // A block of eight waves owns 256 x 256 of the result and a slice of the rows, 32 rows a stage: with 64 x 128 of the result
 // a wave, the LDS reads of a stage (6 KB a wave for 8 MFMAs' worth of a 16-row step) stay below its MFMA time, which a
-// 128 x 128 block of four waves does not reach (8192 rows, 4096 x 4096, bf16 g: 0.91 ms there, 0.35 ms = 790 TFLOP/s here).  The
-// MFMA wants eight consecutive rows of one column in a lane, memory holds rows: a thread loads eight rows of four
-// neighbouring columns, pairs them up by bytes in registers and writes four 16-byte pieces of eight rows each.  Half the
-// threads bring x, half bring g; the stage after the next is in flight from memory while the next is written to the other
-// LDS buffer, one barrier a stage.  The slices' results are added by a second launch in slice order; a grid that fills the
-// chip has one slice and writes the result itself.
+// 128 x 128 block of four waves does not reach (8192 rows, 4096 x 4096, bf16 g: 0.91 ms there, 0.28 ms = 980 TFLOP/s here).
+// The MFMA wants eight consecutive rows of one column in a lane, memory holds rows: a thread loads eight rows of four or
+// eight neighbouring columns, pairs them up by bytes in registers and writes 16-byte pieces of eight rows each.  Half the
+// waves bring x, half bring g; the next stage is written to the other LDS buffer, and the one after that is in flight from
+// memory, while a stage is multiplied; one barrier a stage.  The slices' results are added by a second launch in slice order;
+// a grid that fills the chip has one slice and writes the result itself.
+//
+// What bounds it: many rows and a small result, memory (1.2 M rows, 256 x 172, fp32 g: 4.6 TB/s; at 300 000 rows the slices'
+// partial results and a block's start cost 30 us beside 60 of bytes).  Large results, the chain in a stage: without its
+// loads from memory the 0.28 ms are 0.21, without fragments from LDS 0.24, and the matrix instructions alone take 0.16 (with
+// random operands the chip's power holds them there).  Tried against that chain and slower: three LDS buffers with
+// fragments read across the barrier (0.30), g copied straight to LDS three stages ahead (0.39); all parts dealt out among
+// the matrix instructions gains on wide bf16 (0.26) what it loses where rows are handed on (150 -> 164 us).
 #include <type_traits>
 
 #include "fp8_format.h"

@@ -138,6 +138,22 @@ def dropout_layernorm_relu(z, keep, scale, gamma, beta, eps) -> torch.Tensor:
 
 
 # ------------------------------------------------------- residual stream -> RMS norm -> ReLU
+class _Dropped(torch.autograd.Function):
+    """``z * keep * scale`` in one pass each way (the product of a mask and a number is its own gradient)."""
+
+    @staticmethod
+    def forward(ctx, z, keep, scale):
+        ctx.save_for_backward(keep)
+        ctx.scale = scale
+        return torch.ops.aten.native_dropout_backward(z, keep, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (keep,) = ctx.saved_tensors
+        return torch.ops.aten.native_dropout_backward(g, keep, ctx.scale), None, None
+
+
 class _ResidualRmsNormRelu(torch.autograd.Function):
     """``h = z + residual``, ``relu(rms_norm(h))`` in one pass, the latter written into the right half of a fresh
     ``[N, 2F]`` array (returned whole, the next layer's staged input, in front of ``h``)."""
@@ -597,7 +613,7 @@ class DistSAGE(torch.nn.Module):
                 nodes_feats = dropout_layernorm_relu(z, keep, scale, norm.weight, norm.bias, norm.eps)
                 continue
             if keep is not None:
-                z = z * keep * scale
+                z = _Dropped.apply(z, keep.view(torch.bool), scale)
             after = self.convs[i + 1]
             both = None
             if after.gemm == "fp8" and after.linear_first:  # the normalised rows exist in 8 bits only

@@ -195,3 +195,54 @@ def test_only_what_is_wanted_gets_a_gradient():
     nw = values[2].clone().requires_grad_()
     out, _ = fp8.norm_linear(x, nw, 1e-6, values[3], values[4])
     assert torch.equal(only_norm, torch.autograd.grad((out,), (nw,), (g,))[0])
+
+
+def test_arrays_beyond_2_to_31_elements():
+    """The last rows of arrays of more than 2^31 elements get what they get by themselves (rows do not depend on others; the
+    last 50 000 go through the same kernels as all)."""
+    rows, width, tail = (1 << 23) + 70_001, 256, 50_000
+    assert rows * width > 1 << 31
+    x = torch.empty(rows, width, device="cuda").normal_()
+    nw = torch.rand(width, device="cuda") + 0.5
+    w = fp8.quantize_weight(torch.randn(width, 256, device="cuda") / 16, True)
+    q, part = fp8.quantize_rows(x), fp8.quantize_rows(x[-tail:])
+    same = lambda a, b: torch.equal(a[-tail:].view(torch.uint8), b.view(torch.uint8))  # noqa: E731
+    assert same(q.codes, part.codes) and same(q.scales, part.scales)
+    assert torch.equal(fp8.product(q, w)[-tail:], fp8.product(part, w))
+    assert torch.equal(fp8.product(q, w, out_dtype=torch.bfloat16)[-tail:], fp8.product(part, w, out_dtype=torch.bfloat16))
+    got, h = norm.rms_norm_fp8(x, nw, residual=x, relu=True)
+    want, h_tail = norm.rms_norm_fp8(x[-tail:], nw, residual=x[-tail:], relu=True)
+    assert same(got.codes, want.codes) and same(got.scales, want.scales) and torch.equal(h[-tail:], h_tail)
+    del got, h
+    leaf = x.requires_grad_()
+    y, _ = norm.rms_norm(leaf, nw)
+    (dx,) = torch.autograd.grad((y,), (leaf,), (x.detach(),))
+    small = x.detach()[-tail:].clone().requires_grad_()
+    y_tail, _ = norm.rms_norm(small, nw)
+    (dx_tail,) = torch.autograd.grad((y_tail,), (small,), (small.detach(),))
+    assert torch.equal(y[-tail:], y_tail) and torch.equal(dx[-tail:], dx_tail)
+    del y, dx
+    # columns of g that are one in the last row alone and zero elsewhere: the weight gradient is that row of x
+    g = torch.zeros(rows, width, device="cuda")
+    g[-1] = 1.0
+    dw, db, g_rows = fp8._weight_gradient(q, g, True, True)
+    assert torch.equal(dw, part.dequantize()[-1].unsqueeze(1).expand(width, width)) and bool((db == 1).all())
+    assert same(g_rows.codes, fp8.quantize_rows(g[-tail:]).codes)
+    del q, g_rows
+    # the optimizer, in 32 and in 8 bits (whose second state alone depends on the element's number)
+    x = x.detach().view(-1)
+    at = x.numel() - 5000 // 128 * 128 - x.numel() % 128
+    for bits in (32, 8):
+        def states(n):
+            if bits == 32:
+                return [torch.zeros(n, device="cuda") for _ in "mv"], {}
+            codes = [torch.zeros(n, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in "mv"]
+            scales = [torch.ones(-(-n // 128), dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu) for _ in "mv"]
+            return codes, dict(exp_avg_scales=scales[:1], exp_avg_sq_scales=scales[1:])
+
+        p, p_tail = x.clone(), x[at:].clone()
+        g = g.view(-1).normal_()
+        for param, grad in ((p, g), (p_tail, g[at:])):
+            (m, v), more = states(param.numel())
+            optim.adamw_step([param], [grad], [m], [v], torch.zeros(1, dtype=torch.int32, device="cuda"), lr=0.1, **more)
+        assert torch.equal(p[at:], p_tail)
