@@ -63,6 +63,18 @@ __device__ __forceinline__ f32x4 decode4(uint32_t c) {
     return f32x4{lo.x, lo.y, hi.x, hi.y};
 }
 
+// the largest of 32 neighbouring lanes' words, in all of them
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    // (turned by 1, 2, 4 and 8 lanes inside sixteen, then the sixteens exchanged: on the vector unit, LDS takes no part)
+    const auto larger = [](uint32_t a, int b) { return (uint32_t)b > a ? (uint32_t)b : a; };
+    v = larger(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
+    v = larger(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+    v = larger(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+    v = larger(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));
+    const auto pair = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return pair[0] > pair[1] ? pair[0] : pair[1];
+}
+
 // Four consecutive values of a row of `width`, the first at column c, as they lie in memory (load4_raw: nothing waits for
 // them before widen) or in fp32.  VEC: the row is aligned for one wide load and width % 4 == 0.  Columns past the width
 // read as zero.

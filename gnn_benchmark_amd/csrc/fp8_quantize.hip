@@ -1,6 +1,6 @@
 // Into the 8-bit format (fp8_format.h): rows in blocks of 128 along them, weights in blocks of 128 x 128, stored twice --
 // by output for the forward product, by input for the input gradient.  Streaming kernels, bound by HBM: fp32 rows cost
-// 5 bytes a value, bf16 rows 3 (300 007 x 256 fp32: 86 us = 4.5 TB/s; 8192 x 4096 bf16: 27 us = 3.7 TB/s).
+// 5 bytes a value, bf16 rows 3 (300 007 x 256 fp32: 69 us = 5.6 TB/s; 8192 x 4096 bf16: 21 us = 4.7 TB/s).
 #include <type_traits>
 
 #include "fp8_format.h"
@@ -9,6 +9,7 @@ namespace gnnagg {
 namespace {
 
 // Half a wave owns a block of 128 values of a row, four a lane: one wide load, a maximum over 32 lanes, one 4-byte store.
+// (The maximum on the vector unit: through LDS 63 us against 56 for 300 007 x 172 fp32, 24 against 21 for 8192 x 4096 bf16.)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict__ x, int64_t x_stride,
                                                             uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
@@ -19,10 +20,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict_
         const uint32_t row = id / blocks, block = id - row * blocks;
         const int64_t c = (int64_t)block * kBlock8 + 4 * l;
         const f32x4 v = load4<VEC>(x + (int64_t)row * x_stride, c, width);
-        float top = finite_magnitude(v);
-#pragma unroll
-        for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 32));
-        const int e = block_exponent(top);
+        const int e = block_exponent(__uint_as_float(lanes_max(__float_as_uint(finite_magnitude(v)))));
         reinterpret_cast<uint32_t *>(codes)[(uint64_t)id * 32 + l] = encode4(v, pow2(-e));
         if (l == 0) scales[id] = (uint8_t)(e + 127);
     }

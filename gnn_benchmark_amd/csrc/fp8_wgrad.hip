@@ -222,20 +222,6 @@ struct GRun {
     }
 };
 
-// the largest of 32 neighbouring lanes' words, in all of them
-__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-    auto turned = [&](auto by) {   // by lanes inside sixteen
-        const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + decltype(by)::value, 0xf, 0xf, false);
-        v = other > v ? other : v;
-    };
-    turned(std::integral_constant<int, 1>());
-    turned(std::integral_constant<int, 2>());
-    turned(std::integral_constant<int, 4>());
-    turned(std::integral_constant<int, 8>());
-    const auto pair = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return pair[0] > pair[1] ? pair[0] : pair[1];
-}
-
 // g's rows in the 8-bit format, from the registers on their way to LDS: the input gradient's product wants them, and a pass
 // over g for itself took 65 us (300007 rows of 172, fp32).  A block of 128 columns lies in 32 neighbouring lanes.
 template <typename Run>
