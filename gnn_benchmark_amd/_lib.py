@@ -77,7 +77,7 @@ EXPORTS = (
     "gnnagg_bf16_to_f32",
 )
 
-TRAIN_ABI_VERSION = 2   # GNNAGG_TRAIN_ABI_VERSION of include/gnn_train.h, the second header of the same library
+TRAIN_ABI_VERSION = 1   # GNNAGG_TRAIN_ABI_VERSION of include/gnn_train.h, the second header of the same library
 
 TRAIN_EXPORTS = (
     "gnnagg_train_abi_version",
@@ -90,7 +90,6 @@ TRAIN_EXPORTS = (
     "gnnagg_fp8_product",
     "gnnagg_fp8_weight_gradient_workspace_bytes",
     "gnnagg_fp8_weight_gradient",
-    "gnnagg_fp8_weight_gradient_and_rows",
     "gnnagg_adamw_step",
 )
 
@@ -298,8 +297,6 @@ def _declare_train(L) -> None:
     L.gnnagg_fp8_weight_gradient_workspace_bytes.argtypes = [i64, i64, i64]
     L.gnnagg_fp8_weight_gradient.restype = i32
     L.gnnagg_fp8_weight_gradient.argtypes = [vp, vp, vp, i64, i32, vp, vp, vp, i64, i64, i64, i64, vp]
-    L.gnnagg_fp8_weight_gradient_and_rows.restype = i32
-    L.gnnagg_fp8_weight_gradient_and_rows.argtypes = [vp, vp, vp, i64, i32, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp]
     L.gnnagg_adamw_step.restype = i32
     L.gnnagg_adamw_step.argtypes = [ctypes.POINTER(AdamwTensor), i64, vp, i32, i32, i32, f64, vp, f64, f64, f64, f64,
                                     ctypes.c_uint32, i64, vp]

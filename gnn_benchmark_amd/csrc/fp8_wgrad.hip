@@ -21,7 +21,9 @@
 // loads from memory the 0.28 ms are 0.21, without fragments from LDS 0.24, and the matrix instructions alone take 0.16 (with
 // random operands the chip's power holds them there).  Tried against that chain and slower: three LDS buffers with
 // fragments read across the barrier (0.30), g copied straight to LDS three stages ahead (0.39); all parts dealt out among
-// the matrix instructions gains on wide bf16 (0.26) what it loses where rows are handed on (150 -> 164 us).
+// the matrix instructions gain 6 % on wide bf16 and lose 4 on fp32.  Handing g's rows on in 8 bits from these registers,
+// for the input gradient's product, is no faster than the pass over g that it saves (388 / 391 us for a layer of 300 007 x
+// 256 -> 172 both ways).
 #include <type_traits>
 
 #include "fp8_format.h"
@@ -41,7 +43,6 @@ struct WgradArgs {
     const uint8_t *x, *x_scales;
     const void *g;
     float *out, *bias_out;     // slice 0's result; slice s lies s * k * n (s * n) floats behind
-    uint8_t *g_codes, *g_scales;   // where g's rows go in the 8-bit format, or null
     int64_t g_stride, rows, rows_per_slice, k, n;
     int blocks;                // of 128 along x's rows
     int tiles_n;
@@ -83,8 +84,7 @@ __device__ __forceinline__ uint32_t word(bf16x2_t h) {
 struct Place {                 // of a block and a wave in the result and in the rows
     int64_t k0, n0, begin, end;
     int wk, wn, quarter, lane; // quarter: of the four waves that bring the same operand
-    bool live, sums, rows;     // the wave's part of the result lies inside the matrix; it adds up g's columns; hands on its
-                               // rows in 8 bits
+    bool live, sums;           // the wave's part of the result lies inside the matrix; it adds up g's columns
 };
 
 // What a thread brings of one operand: eight rows of kCols neighbouring columns, in registers as they lie in memory (no
@@ -222,45 +222,6 @@ struct GRun {
     }
 };
 
-// g's rows in the 8-bit format, from the registers on their way to LDS: the input gradient's product wants them, and a pass
-// over g for itself took 65 us (300007 rows of 172, fp32).  A block of 128 columns lies in 32 neighbouring lanes.
-template <typename Run>
-__device__ __forceinline__ void hand_on_rows(const WgradArgs &p, const Place &w, const Run &run, int64_t m0) {
-    const int64_t c = w.n0 + 4 * w.lane, first = m0 + 8 * run.oct;
-    const int64_t blocks = (p.n + kBlock8 - 1) / kBlock8;
-    const bool there = c < blocks * kBlock8;
-    uint8_t *to = p.g_codes + first * blocks * kBlock8 + c;
-    int exponent = 0;                        // of row lane % 8
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-        f32x4 f = run.values(r, 0);
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (c + j >= p.n) f[j] = 0.0f;   // (loads there were of other columns)
-            const uint32_t a = __float_as_uint(f[j]) & 0x7fffffffu;
-            top = a > top ? a : top;
-        }
-        const bool finite = !__any((int)(top >= 0x7f800000u));
-        if (!finite) top = __float_as_uint(finite_magnitude(f));
-        const int e = block_exponent(__uint_as_float(lanes_max(top)));
-        if (w.lane % 8 == r) exponent = e;
-        const float inv = pow2(-e);
-        uint32_t code;
-        if (finite) {
-            const f32x4 v = f * inv;
-            code = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v.x, v.y, 0, false);
-            code = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v.z, v.w, (int)code, true);
-        } else {
-            code = encode4(f, inv);
-        }
-        if (there && first + r < w.end) *reinterpret_cast<uint32_t *>(to) = code;
-        to += blocks * kBlock8;
-    }
-    const int r = w.lane % 32;               // the block's first eight lanes store a row's scale each
-    if (r < 8 && there && first + r < w.end) p.g_scales[(first + r) * blocks + c / kBlock8] = (uint8_t)(exponent + 127);
-}
-
 typedef f32x16 Tiles[4][2];
 
 struct Fragments {             // of one 16-row step: a wave's 128 x 64 of the result
@@ -285,9 +246,6 @@ __device__ __forceinline__ void wgrad_loop(const WgradArgs &p, const Place &w, u
             const int64_t left = w.end - m0 - 8 * run.oct;  // how many of the eight rows are the slice's
 #pragma unroll
             for (int r = 0; r < 8; ++r) run.keep(r, r < left);
-        }
-        if constexpr (!Run::kIsX && Run::kCols == 4) {
-            if (w.rows) hand_on_rows(p, w, run, m0);
         }
 #pragma unroll
         for (int h = 0; h < kTurns; ++h) {
@@ -328,10 +286,9 @@ __device__ __forceinline__ void wgrad_loop(const WgradArgs &p, const Place &w, u
     };
     const std::integral_constant<int, 0> even;
     const std::integral_constant<int, 1> odd;
-    // Stage s lies in LDS buffer s % 3, s + 1 in the next one, its first fragments asked for before the barrier that ends s:
-    // no wave waits for LDS behind a barrier.  s + 2 is written meanwhile, from registers, and the stage that takes these
-    // asked for.  The waves that bring g do that first and multiply behind it, so that their conversions and addresses run
-    // beside the others' matrix instructions, and the other way round.
+    // A stage is multiplied out of one LDS buffer while the next is written to the other, from registers, and the stage that
+    // takes these asked for.  The waves that bring g do that first and multiply behind it, so that their conversions and
+    // addresses run beside the others' matrix instructions, and the other way round.
     uint8_t *now = lds, *next = lds + 2 * kHalfStage;
     auto step = [&](int parity, int64_t m0) {
         if (!Run::kIsX) bring(1 - parity, m0 + kRows, next);
@@ -375,7 +332,6 @@ __global__ __launch_bounds__(512, 2) void fp8_wgrad_kernel(const WgradArgs p) {
     w.end = w.begin + p.rows_per_slice < p.rows ? w.begin + p.rows_per_slice : p.rows;
     w.live = w.k0 + 128 * w.wk < p.k && w.n0 + 64 * w.wn < p.n;
     w.sums = kt == 0 && p.bias_out;
-    w.rows = kt == 0 && p.g_codes;
     const int idx = lane % 32, half = lane / 32;
 
     Tiles acc;
@@ -458,24 +414,13 @@ extern "C" int64_t gnnagg_fp8_weight_gradient_workspace_bytes(int64_t rows, int6
 extern "C" int gnnagg_fp8_weight_gradient(const uint8_t *x, const uint8_t *x_scales, const void *g, int64_t g_stride,
                                           int g_dtype, float *grad_w, float *grad_bias, void *workspace,
                                           int64_t workspace_bytes, int64_t rows, int64_t k, int64_t n, void *stream) {
-    return gnnagg_fp8_weight_gradient_and_rows(x, x_scales, g, g_stride, g_dtype, grad_w, grad_bias, nullptr, nullptr,
-                                               workspace, workspace_bytes, rows, k, n, stream);
-}
-
-extern "C" int gnnagg_fp8_weight_gradient_and_rows(const uint8_t *x, const uint8_t *x_scales, const void *g,
-                                                   int64_t g_stride, int g_dtype, float *grad_w, float *grad_bias,
-                                                   uint8_t *g_codes, uint8_t *g_scales, void *workspace,
-                                                   int64_t workspace_bytes, int64_t rows, int64_t k, int64_t n,
-                                                   void *stream) {
     GNNAGG_REQUIRE(rows >= 0 && k >= 0 && n >= 0, "negative size");
     GNNAGG_REQUIRE(known_dtype(g_dtype), "unknown dtype");
     if (k == 0 || n == 0) return GNNAGG_OK;
     if (!wgrad_sizes_ok(rows, k, n)) return fail(GNNAGG_ERR_UNSUPPORTED, "a weight of %lld x %lld", (long long)k, (long long)n);
     GNNAGG_REQUIRE(grad_w && (rows == 0 || (x && x_scales && g)), "null x/scales/g/grad_w");
     GNNAGG_REQUIRE(g_stride >= n, "a row stride is below the width");
-    GNNAGG_REQUIRE(reinterpret_cast<uintptr_t>(x) % 4 == 0, "codes must be 4-byte aligned");
-    GNNAGG_REQUIRE((g_codes != nullptr) == (g_scales != nullptr), "codes of g without scales, or the other way round");
-    GNNAGG_REQUIRE(reinterpret_cast<uintptr_t>(g_codes) % 4 == 0, "codes of g must be 4-byte aligned");
+    GNNAGG_REQUIRE(reinterpret_cast<uintptr_t>(x) % 8 == 0, "codes must be 8-byte aligned");
     const int64_t slices = wgrad_slices(rows, k, n), need = gnnagg_fp8_weight_gradient_workspace_bytes(rows, k, n);
     GNNAGG_REQUIRE(workspace_bytes >= need && (need == 0 || workspace) && reinterpret_cast<uintptr_t>(workspace) % 4 == 0,
                    "workspace of %lld bytes is too small, null or misaligned", (long long)workspace_bytes);
@@ -483,13 +428,8 @@ extern "C" int gnnagg_fp8_weight_gradient_and_rows(const uint8_t *x, const uint8
     float *bias_parts = !grad_bias ? nullptr : slices == 1 ? grad_bias : parts + slices * k * n;
     const int64_t per = (rows + slices - 1) / slices;
     const int64_t tiles_k = (k + kTile - 1) / kTile, tiles_n = (n + kTile - 1) / kTile;
-    // With one tile along k the pass is bound by memory and the rows' conversion runs beside its loads; with more, the first
-    // tile's blocks alone would convert and the rest wait for them.
-    const bool rows_here = tiles_k == 1;
-    if (g_codes && !rows_here)
-        if (const int rc = gnnagg_fp8_quantize_rows(g, g_stride, g_codes, g_scales, rows, n, g_dtype, stream)) return rc;
-    WgradArgs p{x, x_scales, g, parts, bias_parts, rows_here ? g_codes : nullptr, g_scales, g_stride, rows, (per + kRows - 1) / kRows * kRows, k, n,
-                (int)(pad128(k) / kBlock8), (int)tiles_n};
+    WgradArgs p{x, x_scales, g, parts, bias_parts, g_stride, rows,
+                (per + kRows - 1) / kRows * kRows, k, n, (int)(pad128(k) / kBlock8), (int)tiles_n};
     if (tiles_k * tiles_n > 0x7fffffff) return fail(GNNAGG_ERR_UNSUPPORTED, "too many tiles");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)(tiles_k * tiles_n), (unsigned)slices);
@@ -500,9 +440,9 @@ extern "C" int gnnagg_fp8_weight_gradient_and_rows(const uint8_t *x, const uint8
     const std::integral_constant<int, 4> four;
     const std::integral_constant<int, 8> eight;
     const bool vec = vec4_rows(g, g_stride, n, g_dtype);
-    // (sixteen bytes of bf16 a load where rows allow it and offsets of eight rows fit 32 bits;
-    // where rows are handed on that takes too many registers)
-    const bool wide = g_dtype == GNNAGG_BF16 && !p.g_codes && n % 8 == 0 && g_stride % 8 == 0 && g_stride < (int64_t(1) << 27) &&
+    // Sixteen bytes of bf16 a load where rows allow it and offsets of eight rows fit 32 bits (8192 rows, 4096 x 4096: 299 us
+    // against 319 with eight).
+    const bool wide = g_dtype == GNNAGG_BF16 && n % 8 == 0 && g_stride % 8 == 0 && g_stride < (int64_t(1) << 27) &&
                       reinterpret_cast<uintptr_t>(g) % 16 == 0;
     if (g_dtype == GNNAGG_F32) {
         if (vec) go(float(), four);

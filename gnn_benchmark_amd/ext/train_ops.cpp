@@ -296,9 +296,9 @@ std::tuple<OptTensor, OptTensor, Tensor> public_quantize_weight(const Tensor &w,
     return quantize_weight(w, true, by_input);
 }
 
-// (x^T bf16(g), g's column sums or None, codes and scales of g's rows or None)
-std::tuple<Tensor, OptTensor, OptTensor, OptTensor> weight_gradient(const Tensor &x, const Tensor &x_scales, int64_t k,
-                                                                    const Tensor &g_, bool with_bias, bool with_rows) {
+// (x^T bf16(g), g's column sums or None)
+std::tuple<Tensor, OptTensor> weight_gradient(const Tensor &x, const Tensor &x_scales, int64_t k, const Tensor &g_,
+                                              bool with_bias) {
     check_rows(x, x_scales, k);
     check_gpu(g_, "g", x);
     const int code = dtype_code(g_.scalar_type(), "g");
@@ -308,20 +308,15 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> weight_gradient(const Tensor
     const auto type = x.options().dtype(at::kFloat);
     const int64_t nbytes = gnnagg_fp8_weight_gradient_workspace_bytes(rows, k, n);
     const Tensor grad_w = at::empty({k, n}, type);
-    OptTensor grad_b, codes, scales;
+    OptTensor grad_b;
     if (with_bias) grad_b = at::empty({n}, type);
-    if (with_rows) {
-        auto [c, e] = empty_rows(rows, n, x);
-        codes = c, scales = e;
-    }
     Tensor workspace;
     if (nbytes) workspace = at::empty({nbytes}, type.dtype(at::kByte));
     const Place place(x);
-    check_rc(gnnagg_fp8_weight_gradient_and_rows(
-        bytes(x), bytes(x_scales), g.data, g.stride, code, grad_w.data_ptr<float>(),
-        grad_b ? grad_b->data_ptr<float>() : nullptr, codes ? bytes(*codes) : nullptr, scales ? bytes(*scales) : nullptr,
-        nbytes ? workspace.data_ptr() : nullptr, nbytes, rows, k, n, place.stream));
-    return {grad_w, grad_b, codes, scales};
+    check_rc(gnnagg_fp8_weight_gradient(bytes(x), bytes(x_scales), g.data, g.stride, code, grad_w.data_ptr<float>(),
+                                        grad_b ? grad_b->data_ptr<float>() : nullptr, nbytes ? workspace.data_ptr() : nullptr,
+                                        nbytes, rows, k, n, place.stream));
+    return {grad_w, grad_b};
 }
 
 // (gradient of x and of the residual, gradient of the weight in its type)
@@ -368,21 +363,15 @@ ProductGradients product_gradients(const Tensor &codes, const Tensor &scales, co
                                    int64_t k, const Tensor &g, bool want_x, bool want_w, bool want_b, at::ScalarType x_type,
                                    at::ScalarType w_type, at::ScalarType b_type) {
     ProductGradients grads;
-    const int64_t n = g.size(1);
-    OptTensor g_codes, g_scales;
+    Tensor g_codes, g_scales;
+    if (want_x) std::tie(g_codes, g_scales) = quantize_rows(g);  // (both passes over g beside each other)
     if (want_w || want_b) {  // (the bias's sums come with the weight gradient's pass, beside a frozen weight too)
-        auto [w, b, c, e] = weight_gradient(codes, scales, k, g, want_b, want_x);
+        auto [w, b] = weight_gradient(codes, scales, k, g, want_b);
         if (want_w) grads.w = w.to(w_type);
         if (want_b) grads.b = b->to(b_type);
-        g_codes = c, g_scales = e;
     }
-    if (want_x) {
-        if (!g_codes) {
-            auto [c, e] = quantize_rows(g);
-            g_codes = c, g_scales = e;
-        }
-        grads.x = product(*g_codes, *g_scales, n, by_input, w_scales, k, n, OptTensor(), x_type, OptTensor(), true);
-    }
+    if (want_x)
+        grads.x = product(g_codes, g_scales, g.size(1), by_input, w_scales, k, g.size(1), OptTensor(), x_type, OptTensor(), true);
     return grads;
 }
 

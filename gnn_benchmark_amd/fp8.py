@@ -77,14 +77,8 @@ def product(x: QuantizedRows, weight: QuantizedWeight, bias: Optional[torch.Tens
 
 def weight_gradient(x: QuantizedRows, g: torch.Tensor, with_bias: bool = False):
     """``x^T @ bf16(g)``, fp32 [x.cols, n]; with ``with_bias`` the pair of it and ``g``'s column sums (fp32)."""
-    grad_w, grad_b, _ = _weight_gradient(x, g, with_bias, False)
+    grad_w, grad_b = ext.train_ops().weight_gradient(x.codes, x.scales, x.cols, g, with_bias)
     return (grad_w, grad_b) if with_bias else grad_w
-
-
-def _weight_gradient(x: QuantizedRows, g: torch.Tensor, with_bias: bool, with_rows: bool):
-    """(weight gradient, column sums or None, g in the 8-bit format or None)"""
-    grad_w, grad_b, codes, scales = ext.train_ops().weight_gradient(x.codes, x.scales, x.cols, g, with_bias, with_rows)
-    return grad_w, grad_b, QuantizedRows(codes, scales, g.size(1)) if with_rows else None
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:

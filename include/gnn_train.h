@@ -33,7 +33,7 @@ extern "C" {
 
 /* Raised whenever a prototype of this header changes, comes or goes; bindings compare it with
  * gnnagg_train_abi_version() before the first call. */
-#define GNNAGG_TRAIN_ABI_VERSION 2
+#define GNNAGG_TRAIN_ABI_VERSION 1
 int gnnagg_train_abi_version(void);
 
 /* ---------------------------------------------------------------------------------
@@ -93,12 +93,6 @@ int64_t gnnagg_fp8_weight_gradient_workspace_bytes(int64_t rows, int64_t k, int6
 int gnnagg_fp8_weight_gradient(const uint8_t *x, const uint8_t *x_scales, const void *g, int64_t g_stride, int g_dtype,
                                float *grad_w, float *grad_bias, void *workspace, int64_t workspace_bytes, int64_t rows,
                                int64_t k, int64_t n, void *stream);
-/* The same, and g's rows in the format (codes 4-byte aligned) for the input gradient's product; both NULL: without. */
-int gnnagg_fp8_weight_gradient_and_rows(const uint8_t *x, const uint8_t *x_scales, const void *g, int64_t g_stride,
-                                        int g_dtype, float *grad_w, float *grad_bias, uint8_t *g_codes, uint8_t *g_scales,
-                                        void *workspace, int64_t workspace_bytes, int64_t rows, int64_t k, int64_t n,
-                                        void *stream);
-
 
 /* ---------------------------------------------------------------------------------
  * AdamW (decoupled weight decay) over `count` tensors.  For each: t = ++steps[i];

@@ -308,3 +308,51 @@ def test_a_partition_without_nodes_and_refusals():
     g = torch.randint(-4, 5, (300, 40), device=DEV).float()
     (gb,) = torch.autograd.grad((fp8.linear(x, w.detach(), b),), (b,), (g,))
     assert torch.equal(gb.double(), g.double().sum(0))
+
+
+@pytest.mark.parametrize("linear_first", [False, True])
+@pytest.mark.parametrize("num_bits", [32, 16, 2])
+def test_model_in_evaluation_and_with_narrow_exchanges(linear_first, num_bits):
+    """Without dropout, evaluation gives the training pass's bits where rows travel as they are; with rows of 16 or
+    2 bits a step runs to finite gradients.  Features that are staged or not give the same."""
+    n = 3000
+    part = synthetic.partition_edges(n, 4, 2, 6, 1.8, 800, 1500, 9000, seed=11, device=DEV)
+    graph = synthetic.build_partition_graph(part, 128, True, exchange=synthetic.SeededHaloExchange(4), bits=num_bits,
+                                            device=DEV, exchange_quantized=synthetic.SeededQuantizedHaloExchange(4),
+                                            exchange_bf16=synthetic.SeededBf16HaloExchange(4))
+    torch.manual_seed(0)
+    model = sage.DistSAGE(100, 128, 47, num_layers=3, dropout=0.0, num_bits=num_bits, is_pre_delay=True, gemm="fp8",
+                          norm="rms", linear_first_when_narrowing=linear_first).to(DEV)
+    x = torch.randn(n, 100, device=DEV)
+    out = model.train()(graph, sage.stage_input(x))
+    assert torch.equal(model(graph, x).detach(), out.detach()) and bool(out.isfinite().all())
+    if num_bits == 32:
+        with torch.no_grad():
+            assert torch.equal(model.eval()(graph, x), out.detach())
+    out.square().mean().backward()
+    for name, p in model.named_parameters():
+        assert p.grad is not None and bool(p.grad.isfinite().all()) and bool((p.grad != 0).any()), name
+
+
+def test_degrees_folded_into_the_matrices():
+    """The layer over a graph whose matrices hold the division: the same to rounding, which moves a value to the next code of
+    its block now and then where rows are aggregated before they are quantised (a code's step is 2^-3 of the value at
+    most; a value within 1e-6 of a border between codes is one in 10^5)."""
+    n, fi, fo = 2000, 64, 47
+    graph, _ = partition(n, 2 * fi, True)
+    folded = sage.fold_in_degrees(graph)
+    x = torch.randn(n, fi, device=DEV)
+    g = torch.randn(n, fo, device=DEV)
+    for linear_first in (False, True):
+        torch.manual_seed(1)
+        conv = sage.DistSAGEConvGrad(fi, fo, 32, True, gemm="fp8", linear_first=linear_first).to(DEV)
+        results = []
+        for over in (graph, folded):
+            staged = sage.stage_input(x).requires_grad_()
+            out = conv(over, staged, 0)
+            results.append([out.detach(), *torch.autograd.grad((out,), [staged, *conv.parameters()], (g,))])
+            results[-1][1] = results[-1][1][:, fi:]
+        for a, b in zip(*results):
+            assert float((a - b).norm()) <= 2e-3 * float(a.norm())
+        if linear_first:
+            assert float((results[0][0] - results[1][0]).abs().max()) <= 1e-5 * float(results[0][0].abs().max())
