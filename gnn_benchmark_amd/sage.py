@@ -567,6 +567,8 @@ class DistSAGE(torch.nn.Module):
     stream over the hidden layers and RMS norms in their place.  ``gemm``: the form of the dense products, see
     ``DistSAGEConvGrad``."""
 
+    norm = "layer"   # (of a model stored before there was a choice)
+
     def __init__(self, in_channels, hidden_channels, out_channels, num_layers=3, dropout=0.5, num_bits=32,
                  is_pre_delay=False, linear_first_when_narrowing=False, gemm="fp32", norm="layer"):
         super().__init__()
