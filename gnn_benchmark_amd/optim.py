@@ -38,6 +38,15 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                                exp_avg_scales, exp_avg_sq_scales, seed & 0xFFFFFFFF, first)
 
 
+class _Run:
+    """Parameters of one kind in a group and their array of step counts.  ``kept[i]``: what ``state[params[i]]["step"]`` was
+    made to be, the i-th entry; None while params[i] has no state (its count is zero then)."""
+    __slots__ = ("bits", "params", "steps", "kept")
+
+    def __init__(self, bits: int, params: List[torch.Tensor], steps: torch.Tensor):
+        self.bits, self.params, self.steps, self.kept = bits, params, steps, [None] * len(params)
+
+
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW``'s update and arguments, each parameter group in a few launches.
 
@@ -90,28 +99,43 @@ class AdamW(torch.optim.Optimizer):
             state["master"] = p.detach().float()
         return state
 
+    def _kept_step(self, p: torch.Tensor):
+        """What ``state[p]["step"]`` is; None where p has no state."""
+        state = self.state.get(p)
+        return state.get("step", 0) if state else None
+
     def _prepare(self, index: int, group) -> list:
         """The group's parameters in an order that puts those of one kind (device, type, state) side by side, with one
-        array of step counts for each kind: [(kind, parameters, steps)].  ``state[p]["step"]`` is p's entry of it."""
-        runs = self._runs.get(index)
-        if runs is not None and sum(len(ps) for _, ps, _ in runs) == len(group["params"]):
-            return runs
-        kinds = {}
-        for p in group["params"]:
-            kinds.setdefault(self._kind(p, group), []).append(p)
+        array of step counts for each kind: [_Run].  ``state[p]["step"]`` is p's entry of it.  What a program changes from
+        outside -- parameters, their order, states taken away or put in place, step counts -- is found by comparing with
+        what the arrays were made from, object by object, and the arrays are made again from the states."""
+        ps = group["params"]
+        kinds = [self._kind(p, group) for p in ps]
+        before, known = self._runs.get(index, ([], None))
+        if (known is not None and len(known) == len(ps)
+                and all(p is q and kind == k for p, kind, (q, k) in zip(ps, kinds, known))
+                and all(self._kept_step(p) is kept for run in before for p, kept in zip(run.params, run.kept))):
+            return before
+        by_kind = {}
+        for p, kind in zip(ps, kinds):
+            by_kind.setdefault(kind, []).append(p)
+        if any(kind[0].type != "cuda" for kind in by_kind):
+            raise RuntimeError("Input mismatch: AdamW takes parameters on a GPU (HIP) device")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW's parameters or states are new or were changed: run one step before capturing one")
         runs = []
-        for kind, ps in kinds.items():
-            taken = [self.state[p].get("step", 0) if p in self.state else 0 for p in ps]
-            if kind[0].type != "cuda":
-                raise RuntimeError("Input mismatch: AdamW takes parameters on a GPU (HIP) device")
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("AdamW's states do not exist yet: run one step before capturing one")
-            steps = torch.tensor([int(t) for t in taken], dtype=torch.int32, device=kind[0])
-            for i, p in enumerate(ps):
-                if p in self.state and self.state[p]:
-                    self.state[p]["step"] = steps[i]
-            runs.append((kind, ps, steps))
-        self._runs[index] = runs
+        for kind, members in by_kind.items():
+            steps = torch.tensor([int(self._kept_step(p) or 0) for p in members], dtype=torch.int32, device=kind[0])
+            for old in before:  # the array stays where it is if it can: captured steps raise it there
+                if (old.steps.device == kind[0] and old.bits == kind[2] and len(old.params) == len(members)
+                        and all(p is q for p, q in zip(old.params, members))):
+                    steps = old.steps.copy_(steps)
+            run = _Run(kind[2], members, steps)
+            for i, p in enumerate(members):
+                if self._kept_step(p) is not None:
+                    self.state[p]["step"] = run.kept[i] = run.steps[i]
+            runs.append(run)
+        self._runs[index] = runs, list(zip(ps, kinds))
         return runs
 
     @torch.no_grad()
@@ -122,8 +146,8 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for index, group in enumerate(self.param_groups):
             number = 0
-            for (_, _, bits), ps, steps in self._prepare(index, group):
-                at = 0
+            for run in self._prepare(index, group):
+                ps, at = run.params, 0
                 while at < len(ps):  # stretches of parameters that have a gradient: each has its own count of steps
                     if ps[at].grad is None:
                         at += 1
@@ -131,23 +155,23 @@ class AdamW(torch.optim.Optimizer):
                     end = at
                     while end < len(ps) and ps[end].grad is not None:
                         end += 1
-                    self._step_stretch(group, ps[at:end], steps, at, bits, number + at)
+                    self._step_stretch(group, run, at, end, number + at)
                     at = end
                 number += len(ps)
         return loss
 
-    def _step_stretch(self, group, ps: List[torch.Tensor], steps, at: int, bits: int, number: int) -> None:
-        states = []
-        for i, p in enumerate(ps):
+    def _step_stretch(self, group, run: "_Run", at: int, end: int, number: int) -> None:
+        ps, bits, states = run.params[at:end], run.bits, []
+        for i, p in enumerate(ps, at):
             if p.grad.is_sparse:
                 raise RuntimeError("AdamW does not take sparse gradients")
             state = self.state[p]
             if not state:
                 state.update(self._new_state(p, bits))
-                state["step"] = steps[at + i]
+                state["step"] = run.kept[i] = run.steps[i]
             states.append(state)
         grads = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in ps]
-        adamw_step(ps, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], steps[at:at + len(ps)],
+        adamw_step(ps, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], run.steps[at:end],
                    lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                    masters=[s["master"] for s in states] if ps[0].dtype == torch.bfloat16 else None,
                    exp_avg_scales=[s["exp_avg_scales"] for s in states] if bits == 8 else None,
