@@ -18,6 +18,9 @@ from . import ext
 from .fp8 import BLOCK
 
 _FLOATS = {torch.float32, torch.bfloat16}
+_OWN_KEYS = ("state_bits", "min_8bit_size", "seed")
+# of torch's groups: how its step runs, or (refused unless off) by which rule
+_TORCH_KEYS = ("amsgrad", "maximize", "foreach", "capturable", "differentiable", "fused", "decoupled_weight_decay")
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
@@ -180,30 +183,53 @@ class AdamW(torch.optim.Optimizer):
 
     # ------------------------------------------------------------------ checkpoints
     def load_state_dict(self, state_dict) -> None:
-        """Takes over a ``state_dict`` of this class, or one of ``torch.optim.Adam`` / ``AdamW`` with fp32 states where
-        this optimizer's states are in 32 bits.  (torch's own loading casts states to their parameter's type, which
-        would turn 8-bit codes and fp32 states of bf16 parameters into something else.)"""
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        keep = ("state_bits", "min_8bit_size", "seed")
-        groups = []
-        for g, own in zip(state_dict["param_groups"], self.param_groups):
-            groups.append({**{k: own[k] for k in keep}, **{k: v for k, v in g.items()}})
-        super().load_state_dict({"state": {}, "param_groups": groups if len(groups) == len(state_dict["param_groups"])
-                                 else state_dict["param_groups"]})
-        own = [(p, g) for g in self.param_groups for p in g["params"]]
-        for i, (p, group) in zip(saved, own):
-            old = state_dict["state"].get(i)
-            if not old:
-                continue
-            state = self._new_state(p, self._kind(p, group)[2])
-            for key, t in state.items():
-                src = old.get(key)
-                if key == "master" and src is None:
-                    continue
-                if src is None or src.dtype != t.dtype or src.shape != t.shape:
-                    raise RuntimeError(f"Input mismatch: the saved {key} does not fit this optimizer's states (type and "
-                                       "shape have to be the same)")
-                t.copy_(src)
-            state["step"] = int(old["step"])
-            self.state[p] = state
+        """Takes over a ``state_dict`` of this class, or one of ``torch.optim.AdamW`` (``Adam`` where it has no weight decay)
+        with fp32 states where this optimizer's states are in 32 bits.  Groups that step by another rule -- ``maximize``,
+        ``amsgrad``, a weight decay that is added to the gradient, another class of optimizer -- are refused, and so are states
+        that do not fit; a refusal leaves this optimizer as it was.  (torch's own loading casts states to their parameter's
+        type, which would turn 8-bit codes and fp32 states of bf16 parameters into something else.)"""
+        saved = state_dict["param_groups"]
+        for g in saved:
+            self._refuse_another_rule(g)
+        sizes = [len(g["params"]) for g in saved]
+        if sizes != [len(g["params"]) for g in self.param_groups]:
+            super().load_state_dict({"state": {}, "param_groups": saved})  # says which sizes differ
+        groups = [{**{k: own[k] for k in _OWN_KEYS}, **{k: v for k, v in g.items() if k not in _TORCH_KEYS}}
+                  for g, own in zip(saved, self.param_groups)]
+        states = {}
+        for g, own in zip(groups, self.param_groups):
+            for i, p in zip(g["params"], own["params"]):
+                old = state_dict["state"].get(i)
+                if old:
+                    states[p] = self._taken_over(old, self._new_state(p, self._kind(p, g)[2]))
+        super().load_state_dict({"state": {}, "param_groups": groups})
+        self.state.update(states)
         self._runs = {}
+
+    @staticmethod
+    def _refuse_another_rule(group) -> None:
+        if "state_bits" in group:  # this class's
+            return
+        why = None
+        if "amsgrad" not in group or "betas" not in group:
+            why = "not torch.optim.Adam's or AdamW's"
+        elif group["amsgrad"] or group.get("maximize"):
+            why = "amsgrad" if group["amsgrad"] else "maximize"
+        elif group["weight_decay"] != 0 and group.get("decoupled_weight_decay") is False:
+            why = "a weight decay that is added to the gradient"
+        if why:
+            raise RuntimeError(f"Input mismatch: the saved parameter groups step by another rule ({why})")
+
+    @staticmethod
+    def _taken_over(old, state: dict) -> dict:
+        """The saved state ``old`` in the place of the fresh one."""
+        for key, t in state.items():
+            src = old.get(key)
+            if key == "master" and src is None:
+                continue
+            if src is None or src.dtype != t.dtype or src.shape != t.shape:
+                raise RuntimeError(f"Input mismatch: the saved {key} does not fit this optimizer's states (type and "
+                                   "shape have to be the same)")
+            t.copy_(src)
+        state["step"] = int(old["step"])
+        return state
