@@ -534,19 +534,31 @@ void same_sizes(const Tensors &tensors, const Tensors &params, const char *what,
                                               : " does not hold one value for each 128 elements of its state");
 }
 
-// No byte may be written twice: two blocks would race for it.
-void refuse_overlaps(std::initializer_list<const Tensors *> lists) {
-    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-    for (const Tensors *tensors : lists)
+typedef std::pair<uintptr_t, uintptr_t> Span;  // of addresses, the end behind it
+
+Span span_of(const Tensor &t) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    return {at, at + t.nbytes()};
+}
+
+// No byte may be written twice, and none that is written may be read as something else: blocks would race for it.
+void refuse_overlaps(std::initializer_list<const Tensors *> written, std::initializer_list<const Tensors *> read) {
+    std::vector<Span> spans;
+    for (const Tensors *tensors : written)
         for (const Tensor &t : *tensors)
-            if (t.numel() > 0) {
-                const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-                spans.emplace_back(at, at + t.nbytes());
-            }
+            if (t.numel() > 0) spans.push_back(span_of(t));
     std::sort(spans.begin(), spans.end());
     for (size_t i = 1; i < spans.size(); ++i)
         TORCH_CHECK(spans[i].first >= spans[i - 1].second,
                     "Input mismatch: the same memory twice among parameters, states, masters and steps");
+    for (const Tensors *tensors : read)
+        for (const Tensor &t : *tensors) {
+            if (t.numel() == 0) continue;
+            const Span s = span_of(t);
+            const auto behind = std::lower_bound(spans.begin(), spans.end(), Span{s.second, 0});  // first that starts behind s
+            TORCH_CHECK(behind == spans.begin() || std::prev(behind)->second <= s.first,
+                        "Input mismatch: a gradient or the learning rate in the same memory as what the step writes");
+        }
 }
 
 void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_avgs, const Tensors &exp_avg_sqs,
@@ -602,7 +614,9 @@ void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_
         lr = lr_.cast<double>();
     }
     const Tensors step_list = {steps};
-    refuse_overlaps({&params, &exp_avgs, &exp_avg_sqs, &masters, &m_scales, &v_scales, &step_list});
+    Tensors rate;
+    if (lr_tensor.defined()) rate.push_back(lr_tensor);
+    refuse_overlaps({&params, &exp_avgs, &exp_avg_sqs, &masters, &m_scales, &v_scales, &step_list}, {&grads, &rate});
     std::vector<gnnagg_adamw_tensor> records(count);
     for (size_t i = 0; i < count; ++i) {
         gnnagg_adamw_tensor &r = records[i];

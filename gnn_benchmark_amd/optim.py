@@ -35,8 +35,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     rounded).  Gradients: all fp32 or all bf16.  States: fp32 ``exp_avgs`` / ``exp_avg_sqs``, or float8_e4m3fn codes of m
     and sqrt(v) with ``exp_avg_scales`` / ``exp_avg_sq_scales`` (float8_e8m0fnu, one for each 128 elements).  ``lr``: a
     number, or an fp32 scalar on the device that is read when the step runs.  No tensor that is written may overlap another
-(that is refused).  ``first``: number of the first tensor for
-    the 8-bit states' random bits, where a list is split over calls."""
+    that is written or read, gradients and a learning rate on the device among them (that is refused).  ``first``: number
+    of the first tensor for the 8-bit states' random bits, where a list is split over calls."""
     ext.train_ops().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas[0], betas[1], eps, weight_decay, masters,
                                exp_avg_scales, exp_avg_sq_scales, seed & 0xFFFFFFFF, first)
 

@@ -109,7 +109,8 @@ int gnnagg_fp8_weight_gradient(const uint8_t *x, const uint8_t *x_scales, const 
  *     of (seed, first + i, t, j): equal calls give equal results.  `first`: the number of the first tensor, for callers
  *     that split a list over several calls.
  * steps: int32 [count] on the device, the number of steps taken so far, raised by one here: a captured call counts its
- * replays.  lr_tensor: fp32 scalar on the device that is read instead of lr, or NULL.
+ * replays.  lr_tensor: fp32 scalar on the device that is read instead of lr, or NULL.  No memory that is written may
+ * overlap any other that is written or read here (not checked at this level).
  * ------------------------------------------------------------------------------- */
 typedef struct gnnagg_adamw_tensor {
     void *param;
