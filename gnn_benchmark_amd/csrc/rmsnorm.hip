@@ -132,8 +132,9 @@ __device__ __forceinline__ void inverse_rms(const f32x4 (&h)[U][NV], double inv_
     for (int u = 0; u < U; ++u) {
         // 1 / sqrt: the hardware's estimate (2^-26) and a Newton step, beyond fp32 by far.  The library's square root and
         // division in 64 bits are some 60 instructions (8192 x 5120 bf16, forward: 103 us with them, 88 without).
-        const double a = q[u] * inv_width + eps, y = __builtin_amdgcn_rsq(a);
-        r[u] = (float)(y * __builtin_fma(-0.5 * a * y, y, 1.5));
+        // (An infinite a has the root's inverse 0, a zero one infinity, and the step would make NaN of either.)
+        const double a = q[u] * inv_width + eps, y = __builtin_amdgcn_rsq(a), step = __builtin_fma(-0.5 * a * y, y, 1.5);
+        r[u] = (float)(step == step ? y * step : y);
     }
 }
 

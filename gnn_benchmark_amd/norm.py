@@ -1,7 +1,8 @@
 """RMS norm with the residual's addition, in one pass each way: ``h = x + residual``,
 ``y = relu?(h / sqrt(mean(h^2) + eps) * weight)`` -- next to ``sage.dropout_layernorm_relu``, for layers that carry a
 residual stream -- and the same with ``y`` leaving in the 8-bit format that ``fp8.product`` reads.  Widths of 1 to 16384,
-fp32 or bf16 rows, the weight in fp32 or the rows' type."""
+fp32 or bf16 rows, the weight in fp32 or the rows' type.  In a row with an infinity ``1 / sqrt(mean(h^2) + eps)`` is zero: its
+finite values give zero, its infinite ones NaN; a NaN makes its whole row NaN, and either spoils no other row."""
 from typing import Optional, Tuple
 
 import torch

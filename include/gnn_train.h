@@ -40,7 +40,8 @@ int gnnagg_train_abi_version(void);
  * RMS norm with the residual's addition, rows of `width` <= 16384 values:
  *   h = x + residual (rounded to dtype; h = x where residual is NULL)
  *   y = h / sqrt(mean(h^2) + eps) * weight, then max(y, 0) where relu != 0
- * The mean square is summed in 64 bits, the rest is fp32.
+ * The mean square is summed in 64 bits, the rest is fp32.  In a row with an infinity the inverse root is zero: its finite
+ * values give zero, its infinite ones NaN.  A NaN makes its whole row NaN.
  *   x, residual (or NULL), h (written where residual is given, NULL otherwise), y: dtype, row strides of their own
  *   weight: [width], weight_dtype GNNAGG_F32 or dtype
  * ------------------------------------------------------------------------------- */
