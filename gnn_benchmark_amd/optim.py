@@ -147,8 +147,8 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        number = 0  # of a tensor among all groups', for its random bits
         for index, group in enumerate(self.param_groups):
-            number = 0
             for run in self._prepare(index, group):
                 ps, at = run.params, 0
                 while at < len(ps):  # stretches of parameters that have a gradient: each has its own count of steps
