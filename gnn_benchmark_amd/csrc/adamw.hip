@@ -35,7 +35,9 @@ __global__ void raise_steps_kernel(int32_t *steps, int64_t n) {
     if (i < n) steps[i] += 1;
 }
 
-// 20 random bits of element j: a multiply-xorshift hash of j and the key of (seed, tensor, step)
+// 20 random bits of element j: a multiply-xorshift hash of j and the key of (seed, tensor, step).  The multipliers are
+// published ones: the first two from C. Wellons' search for 32-bit hashes of low bias, the third a prime of Y. Collet's; the
+// key's are 2^32 over the golden ratio and one of A. Appleby's.
 __device__ __forceinline__ uint32_t random20(uint32_t key, uint32_t j) {
     uint32_t x = (j ^ key) * 0x7FEB352Du;
     x = (x ^ (x >> 15)) * 0x846CA68Bu;
