@@ -143,6 +143,10 @@ class _Dropped(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, z, keep, scale):
+        if keep.dtype not in (torch.bool, torch.uint8) or keep.shape != z.shape or keep.device != z.device:
+            raise RuntimeError("Input mismatch: keep must be a bool/uint8 mask shaped like z, on its device")
+        if keep.dtype == torch.uint8:  # (any byte but zero keeps; as bits of a bool only 0 and 1 have a meaning)
+            keep = keep != 0
         ctx.save_for_backward(keep)
         ctx.scale = scale
         return torch.ops.aten.native_dropout_backward(z, keep, scale)
@@ -615,7 +619,7 @@ class DistSAGE(torch.nn.Module):
                 nodes_feats = dropout_layernorm_relu(z, keep, scale, norm.weight, norm.bias, norm.eps)
                 continue
             if keep is not None:
-                z = _Dropped.apply(z, keep.view(torch.bool), scale)
+                z = _Dropped.apply(z, keep, scale)
             after = self.convs[i + 1]
             both = None
             if after.gemm == "fp8" and after.linear_first:  # the normalised rows exist in 8 bits only
