@@ -319,6 +319,12 @@ std::tuple<Tensor, OptTensor> weight_gradient(const Tensor &x, const Tensor &x_s
     return {grad_w, grad_b};
 }
 
+std::tuple<Tensor, OptTensor> public_weight_gradient(const Tensor &x, const Tensor &x_scales, int64_t k, const Tensor &g,
+                                                     bool with_bias) {
+    if (at::GradMode::is_enabled()) refuse_grad(g);
+    return weight_gradient(x, x_scales, k, g, with_bias);
+}
+
 // (gradient of x and of the residual, gradient of the weight in its type)
 std::tuple<Tensor, Tensor> rms_norm_backward(const Tensor &grad_y_, const OptTensor &grad_h_, const Tensor &h_,
                                              const Tensor &weight_, double eps, bool relu) {
@@ -656,7 +662,7 @@ PYBIND11_MODULE(train_ops, m) {
     m.def("quantize_rows", &public_quantize_rows);
     m.def("quantize_weight", &public_quantize_weight);
     m.def("product", &public_product);
-    m.def("weight_gradient", &weight_gradient);
+    m.def("weight_gradient", &public_weight_gradient);
     m.def("linear", &linear);
     m.def("norm_linear", &norm_linear);
     m.def("adamw_step", &adamw_step);

@@ -76,7 +76,8 @@ def product(x: QuantizedRows, weight: QuantizedWeight, bias: Optional[torch.Tens
 
 
 def weight_gradient(x: QuantizedRows, g: torch.Tensor, with_bias: bool = False):
-    """``x^T @ bf16(g)``, fp32 [x.cols, n]; with ``with_bias`` the pair of it and ``g``'s column sums (fp32)."""
+    """``x^T @ bf16(g)``, fp32 [x.cols, n]; with ``with_bias`` the pair of it and ``g``'s column sums (fp32).
+    No gradient."""
     grad_w, grad_b = ext.train_ops().weight_gradient(x.codes, x.scales, x.cols, g, with_bias)
     return (grad_w, grad_b) if with_bias else grad_w
 
