@@ -3,9 +3,9 @@
 //     grad_w[k, n] = sum over rows m of x[m, k] * bf16(g[m, n]),   grad_bias[n] = sum over rows of g[m, n],
 //
 // x in the 8-bit format.  A scale of that format varies along the contraction here, so it cannot be left to the matrix
-// unit; but a code times a power of two is a bf16 value, so x is turned into bf16 exactly on its way into LDS and the
-// product runs on the bf16 matrix units: x loses nothing, g is rounded to 8 significant bits, sums are fp32.  What the
-// forward has to keep for it is one byte a value.
+// unit; but a code times a power of two in [2^-124, 2^119] is a bf16 value, so x is turned into bf16 exactly on its way into
+// LDS (beyond these, to bf16's subnormals and infinity) and the product runs on the bf16 matrix units: x loses nothing, g is
+// rounded to 8 significant bits, sums are fp32.  What the forward has to keep for it is one byte a value.
 //
 // A block of eight waves owns 256 x 256 of the result and a slice of the rows, 32 rows a stage: with 64 x 128 of the result
 // a wave, the LDS reads of a stage (6 KB a wave for 8 MFMAs' worth of a 16-row step) stay below its MFMA time, which a

@@ -77,7 +77,10 @@ int gnnagg_fp8_quantize_rows(const void *x, int64_t x_stride, uint8_t *codes, ui
 int gnnagg_fp8_quantize_weight(const void *w, int64_t w_stride, uint8_t *codes_by_output, uint8_t *codes_by_input,
                                uint8_t *scales, int64_t k, int64_t n, int dtype, void *stream);
 
-/* out[m, n] = sum_k x[m, k] w[n, k] (+ bias[n]), fp32 accumulation, stored as out_dtype:
+/* out[m, n] = sum_k x[m, k] w[n, k] (+ bias[n]), accumulated in fp32, stored as out_dtype.  GNNAGG_F32: products exact, for
+ * scales in [2^-124, 2^119] (below, the smallest codes are rounded to bf16's subnormals; 2^128 is infinite).  GNNAGG_BF16: of the
+ * products of eight neighbouring codes each is cut to a multiple of 2^-13 of the largest one's power of two (the 8-bit
+ * matrix instruction's way), at any scale.
  *   x codes [rows][k padded] with scales [rows][k padded / 128]; w codes [n][k padded] whose block (kb, nb) has the
  *   scale w_scales[kb * scale_k_stride + nb * scale_n_stride]; bias fp32 [n] or NULL; out row stride out_stride.
  * Codes and padding are read whole: 16-byte aligned, k padded to a multiple of 128.  The forward product takes the codes
@@ -86,8 +89,8 @@ int gnnagg_fp8_product(const uint8_t *x, const uint8_t *x_scales, const uint8_t 
                        int64_t scale_k_stride, int64_t scale_n_stride, const float *bias, void *out, int64_t out_stride,
                        int out_dtype, int64_t rows, int64_t k, int64_t n, void *stream);
 
-/* grad_w[k, n] = sum_m x[m, k] * bf16(g[m, n]) in fp32 (x: the format's rows; every value of the format times its scale
- * is a bf16 value, so x enters exactly) and, where grad_bias is not NULL, grad_bias[n] = sum_m g[m, n] in fp32.
+/* grad_w[k, n] = sum_m x[m, k] * bf16(g[m, n]) in fp32 (x: the format's rows; a code times a scale in [2^-124, 2^119] is a
+ * bf16 value, so x enters exactly; outside as for the fp32 product) and, where grad_bias is not NULL, grad_bias[n] = sum_m g[m, n] in fp32.
  * g: g_dtype, row stride g_stride.  grad_w fp32 [k][n].  workspace: gnnagg_fp8_weight_gradient_workspace_bytes (checked),
  * any contents. */
 int64_t gnnagg_fp8_weight_gradient_workspace_bytes(int64_t rows, int64_t k, int64_t n);
