@@ -192,6 +192,26 @@ std::tuple<Tensor, Tensor> quantize_rows(const Tensor &x) {
     return {codes, scales};
 }
 
+typedef std::pair<uintptr_t, uintptr_t> Span;  // of addresses, the end behind it
+
+Span span_of(const Tensor &t) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    return {at, at + t.nbytes()};
+}
+
+// Whether a contiguous operand shares bytes with rows [rows, cols] of `out`; columns of a wider array beside them do not
+// count.
+bool shares_memory(const Tensor &out, const Tensor &operand) {
+    if (out.numel() == 0 || operand.numel() == 0) return false;
+    const Span s = span_of(operand);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(out.const_data_ptr()), size = out.element_size();
+    const uintptr_t width = size * out.size(1), pitch = out.size(0) > 1 ? size * out.stride(0) : width;
+    if (s.second <= at || s.first >= at + (out.size(0) - 1) * pitch + width) return false;
+    if (s.first < at) return true;
+    const uintptr_t in_row = (s.first - at) % pitch;       // the row that s begins in, or behind
+    return in_row < width || s.first - in_row + pitch < s.second;
+}
+
 void check_rows(const Tensor &codes, const Tensor &scales, int64_t cols) {
     check_gpu(codes, "x");
     check_gpu(scales, "x' scales", codes);
@@ -233,6 +253,8 @@ Tensor product(const Tensor &x, const Tensor &x_scales, int64_t cols, const OptT
         check_gpu(*out_, "out", x);
         TORCH_CHECK(out_->dim() == 2 && out_->size(0) == rows && out_->size(1) == wide && rows_lie_dense(*out_),
                     "Input mismatch: out must be [rows, outputs] with contiguous rows");
+        for (const Tensor *t : std::initializer_list<const Tensor *>{&x, &x_scales, &*w_codes, &w_scales, &bias})
+            TORCH_CHECK(!t->defined() || !shares_memory(*out_, *t), "Input mismatch: out shares memory with an operand");
     }
     const Tensor out = out_ ? *out_ : at::empty({rows, wide}, x.options().dtype(out_dtype));
     const Place place(x);
@@ -538,13 +560,6 @@ void same_sizes(const Tensors &tensors, const Tensors &params, const char *what,
         TORCH_CHECK(tensors[i].numel() == (params[i].numel() + block - 1) / block, "Input mismatch: ", what,
                     " number ", i, block == 1 ? " has another size than its parameter"
                                               : " does not hold one value for each 128 elements of its state");
-}
-
-typedef std::pair<uintptr_t, uintptr_t> Span;  // of addresses, the end behind it
-
-Span span_of(const Tensor &t) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-    return {at, at + t.nbytes()};
 }
 
 // No byte may be written twice, and none that is written may be read as something else: blocks would race for it.
