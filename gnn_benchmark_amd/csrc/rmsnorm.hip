@@ -343,22 +343,23 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_backward_kernel(const 
     }
 }
 
-// 32 columns a block, 32 slices of the partial rows, added in slice order
+// 32 columns a block, 32 slices of the partial rows, added in slice order, in 64 bits (hidden behind the loads; in 32 the
+// chain would be as long as a thread's own over its rows)
 __global__ __launch_bounds__(1024) void column_reduce_kernel(const float *__restrict__ partial, int64_t blocks,
                                                              int64_t width, float *__restrict__ out) {
-    __shared__ float sums[32][33];
+    __shared__ double sums[32][33];
     const int col = (int)threadIdx.x % 32, slice = (int)threadIdx.x / 32;
     const int64_t c = (int64_t)blockIdx.x * 32 + col;
-    float a = 0.0f;
+    double a = 0.0;
     if (c < width) {
 #pragma unroll 8
-        for (int64_t b = slice; b < blocks; b += 32) a += partial[b * width + c];
+        for (int64_t b = slice; b < blocks; b += 32) a += (double)partial[b * width + c];
     }
     sums[slice][col] = a;
     __syncthreads();
     if (slice == 0 && c < width) {
         for (int q = 1; q < 32; ++q) a += sums[q][col];
-        out[c] = a;
+        out[c] = (float)a;
     }
 }
 
