@@ -14,7 +14,7 @@
 //          (2e-8 off on the same operands), at half the matrix rate.
 //
 // Large bf16 products are bound by the matrix unit as far as its power allows (8192^3: 0.61 ms = 1.81 PFLOP/s, with neither
-// scales nor copies 0.40), products of many rows with a small weight by memory (1 M x 512 x 256 to fp32: 0.34 ms), single
+// scales nor copies 0.40; to fp32 0.91 ms = 1.21 PFLOP/s), products of many rows with a small weight by memory (1 M x 512 x 256 to fp32: 0.34 ms), single
 // tokens by the launch and the weight's bytes (1 x 4096 x 4096: 5 us on the GPU, 6 from call to call).
 //
 // Both operands have the contraction index contiguous.  A pipeline stage is half a block of it, 64 bytes of every row of the
@@ -533,9 +533,11 @@ template <typename O>
 int launch_product(const ProductArgs &p, hipStream_t st) {
     const int64_t columns = (p.n + 15) / 16;
     // Few rows, or a small result: the tiled kernel would have a block for each 128 columns and rows only, this one has one
-    // for each 16 columns and 64 rows (to fp32, this kernel / tiles: 65 x 1024 x 1024 5 / 13 us, 300 x 512 x 256 4 / 9 us,
-    // 128 x 4096 x 4096, two blocks a compute unit, 28 / 36 us, 300 x 4096 x 4096 67 / 38 us).
-    if (p.rows <= 64 || columns * ((p.rows + 63) / 64) <= 256) {
+    // for each 16 columns and 64 rows, up to two a compute unit (to bf16 unless said otherwise, this kernel / tiles:
+    // 65 x 1024 x 1024 4.6 / 8.1 us, 300 x 512 x 256 3.6 / 6.7, 4000 x 128 x 128 3.3 / 5.4, 512 blocks: 2000 x 512 x 256
+    // 5.0 / 6.8, 128 x 4096 x 4096 27 / 27 and to fp32 27 / 34, 512 x 4096 x 1024 27 / 27 and 27 / 34; 1000 blocks:
+    // 4000 x 512 x 256 7.9 / 7.0, 256 x 4096 x 4096 52 / 27, 8000 x 128 x 128 4.5 / 5.5).
+    if (p.rows <= 64 || columns * ((p.rows + 63) / 64) <= 512) {
         auto few = [&](auto mt) {
             constexpr int kMt = decltype(mt)::value;
             hipLaunchKernelGGL((fp8_product_few_kernel<O, kMt>),
@@ -547,19 +549,26 @@ int launch_product(const ProductArgs &p, hipStream_t st) {
         GNNAGG_HIP(hipGetLastError());
         return GNNAGG_OK;
     }
-    // Many rows against a weight that fits LDS: below about 40 000 rows bringing the weight there costs more than it saves
-    // (512 x 256 to fp32, this kernel / tiles: 20 000 rows 19 / 17 us, 65 536 rows 30 / 35 us, 1 M rows 0.34 / 0.64 ms).
-    if (p.rows >= 40000 && rows_lds(p)) {
+    // Many rows against a weight that fits LDS: one of up to 128 columns is there at once, a wider one costs more to bring
+    // than it saves below about 20 000 rows (this kernel / tiles, bf16 and fp32: 4500 rows 256 x 128 4.9 / 5.8 and 5.8 / 6.7 us,
+    // 512 x 128 5.6 / 6.8 and 7.0 / 8.4; 9000 rows 256 x 256 7.2 / 6.4 and 9.4 / 7.8; 16 000 rows 256 x 256 7.7 / 7.4 and
+    // 11.0 / 9.8, 512 x 256 10.6 / 9.4 and 14.6 / 12.0; 20 000 rows 256 x 256 8.3 / 9.5 and 11.6 / 12.1, 512 x 256 11.7 / 12.1
+    // and 15.3 / 15.0, 256 x 172 7.9 / 8.4 and 10.8 / 11.2; 60 000 rows 512 x 256 17 / 23 and 25 / 32; 1 M rows 512 x 256
+    // to fp32 0.34 / 0.64 ms).
+    if ((p.rows >= 20000 || p.n <= kBlock8) && rows_lds(p)) {
         if (p.blocks == 1) return launch_rows<O, 1>(p, st);
         if (p.blocks == 2) return launch_rows<O, 2>(p, st);
         if (p.blocks == 3) return launch_rows<O, 3>(p, st);
         return launch_rows<O, 4>(p, st);
     }
     // Tiles of 256 x 256 feed the matrix units better, but a compute unit holds one block of them and nothing runs beside its
-    // start and end: they pay where the contraction is long and there are two rounds of them (to bf16, 256 / 128:
-    // 8192^3 0.61 / 0.78 ms, 8192 x 4096 x 4096 180 / 178 us, 4096^3 95 / 92 us, 100 000 x 1024 x 1024 253 / 233 us).
-    const int64_t large = ((p.rows + 255) / 256) * ((p.n + 255) / 256);
-    if (p.blocks >= 32 && large >= 512) return launch_tiles<O, 4, 4, 2, 2>(p, st);
+    // start and end: they pay where the contraction is long and the last round of blocks is nearly full (256 / 128, bf16 and
+    // fp32: 8192^3 599 / 665 and 906 / 972 us, 8192 x 16384 x 2048 269 / 337 and 400 / 495, 9000 x 5120 x 5120 252 / 313 and
+    // 401 / 443, 4096^3 81 / 80 and 114 / 129, 8192 x 4096 x 4096 188 / 185 and 234 / 263; rounds a quarter empty: 6000^3 259 / 273
+    // and 444 / 392, 5000 x 4096 x 4096 129 / 103 and 208 / 159; short contractions: 8192 x 2048 x 4096 118 / 88 and 145 / 149,
+    // 100 000 x 1024 x 1024 218 / 203 and 291 / 278).
+    const int64_t large = ((p.rows + 255) / 256) * ((p.n + 255) / 256), rounds = (large + 255) / 256;
+    if (p.blocks >= 32 && 10 * large >= 9 * 256 * rounds) return launch_tiles<O, 4, 4, 2, 2>(p, st);
     return launch_tiles<O, 2, 2, 2, 2>(p, st);
 }
 
