@@ -1,6 +1,8 @@
 // Into the 8-bit format (fp8_format.h): rows in blocks of 128 along them, weights in blocks of 128 x 128, stored twice --
 // by output for the forward product, by input for the input gradient.  Streaming kernels, bound by HBM: fp32 rows cost
-// 5 bytes a value, bf16 rows 3 (300 007 x 256 fp32: 69 us = 5.6 TB/s; 8192 x 4096 bf16: 21 us = 4.7 TB/s).
+// 5 bytes a value, bf16 rows 3 (with four operands in turn: 300 007 x 256 fp32 68 us = 5.6 TB/s, x 172 52 us, 8192 x 4096 bf16
+// 24 us = 4.2 TB/s, a bf16 weight of 4096 x 4096 in both orders 17 us; inside a layer's pass, behind kernels whose results
+// are still being written back, 87 us for the first two on average, 25 and 25).
 #include <type_traits>
 
 #include "fp8_format.h"
@@ -9,7 +11,8 @@ namespace gnnagg {
 namespace {
 
 // Half a wave owns a block of 128 values of a row, four a lane: one wide load, a maximum over 32 lanes, one 4-byte store.
-// (The maximum on the vector unit: through LDS 63 us against 56 for 300 007 x 172 fp32, 24 against 21 for 8192 x 4096 bf16.)
+// (The maximum on the vector unit: through LDS 63 us against 56 for 300 007 x 172 fp32, 24 against 21 for 8192 x 4096 bf16,
+// each on one operand again and again.)
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T *__restrict__ x, int64_t x_stride,
                                                             uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,

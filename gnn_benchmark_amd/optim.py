@@ -183,8 +183,8 @@ class AdamW(torch.optim.Optimizer):
 
     # ------------------------------------------------------------------ checkpoints
     def load_state_dict(self, state_dict) -> None:
-        """Takes over a ``state_dict`` of this class, or one of ``torch.optim.AdamW`` (``Adam`` where it has no weight decay)
-        with fp32 states where this optimizer's states are in 32 bits.  Groups that step by another rule -- ``maximize``,
+        """Takes over a ``state_dict`` of this class, or one of ``torch.optim.AdamW`` (``Adam`` where it has no weight decay;
+        groups of a torch that does not say how its decay works are taken for AdamW's) with fp32 states where this optimizer's states are in 32 bits.  Groups that step by another rule -- ``maximize``,
         ``amsgrad``, a weight decay that is added to the gradient, another class of optimizer -- are refused, and so are states
         that do not fit; a refusal leaves this optimizer as it was.  (torch's own loading casts states to their parameter's
         type, which would turn 8-bit codes and fp32 states of bf16 parameters into something else.)"""
