@@ -55,7 +55,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits`` 8 keeps both states of tensors of at least ``min_8bit_size`` elements in 8 bits (2 bytes an element
     instead of 8), the others in 32.  bf16 parameters keep an fp32 master in their state.  A step can be captured into a
-    HIP graph once it has run eagerly (the states exist then); ``lr`` may be an fp32 scalar tensor on the device, which a
+    HIP graph once it has run eagerly (the states exist then; a parameter, state or step count that a program changes is found
+    by the next step, which has to be an eager one); ``lr`` may be an fp32 scalar tensor on the device, which a
     captured step reads anew at every replay.  Sparse gradients are refused."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits: int = 32,
