@@ -78,7 +78,8 @@ def product(x: QuantizedRows, weight: QuantizedWeight, bias: Optional[torch.Tens
     """``x @ weight (+ bias)`` of 8-bit operands, [rows, n] in ``out_dtype``: float32, products exact and sums in
     fp32; or bfloat16, through the 8-bit instruction, whose cut of neighbouring products is described above.
     ``input_gradient``: ``x @ weight^T``, [rows, k], from the codes by input.  ``out``: an array of that shape with
-    contiguous rows (a column block of a wider one is fine) to write into, apart from the operands' memory.  No gradient (``linear`` has one)."""
+    contiguous rows (a column block of a wider one is fine) to write into, apart from the operands' memory.  No gradient
+    (``linear`` has one)."""
     return ext.train_ops().product(x.codes, x.scales, x.cols, weight.codes_by_input if input_gradient else weight.codes,
                                    weight.scales, weight.k, weight.n, bias, out_dtype, out, input_gradient)
 

@@ -55,9 +55,9 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits`` 8 keeps both states of tensors of at least ``min_8bit_size`` elements in 8 bits (2 bytes an element
     instead of 8), the others in 32.  bf16 parameters keep an fp32 master in their state.  A step can be captured into a
-    HIP graph once it has run eagerly (the states exist then; a parameter, state or step count that a program changes is found
-    by the next step, which has to be an eager one); ``lr`` may be an fp32 scalar tensor on the device, which a
-    captured step reads anew at every replay.  Sparse gradients are refused."""
+    HIP graph once it has run eagerly (the states exist then); ``lr`` may be an fp32 scalar tensor on the device, which a
+    captured step reads anew at every replay.  A parameter, state or step count that a program changes is found by the next
+    step, which has to be an eager one; steps captured before go on as they were.  Sparse gradients are refused."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits: int = 32,
                  min_8bit_size: int = 4096, seed: int = 0):
@@ -69,13 +69,13 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"Invalid betas: {betas}")
         if eps < 0.0 or weight_decay < 0.0:
             raise ValueError("eps and weight_decay must not be negative")
-        self._runs = {}
+        self._runs, self._captured = {}, []
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
                                       state_bits=state_bits, min_8bit_size=min_8bit_size, seed=seed))
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._runs = {}
+        self._runs, self._captured = {}, []
 
     # ------------------------------------------------------------------ states
     @staticmethod
@@ -174,6 +174,8 @@ class AdamW(torch.optim.Optimizer):
                 state.update(self._new_state(p, bits))
                 state["step"] = run.kept[i] = run.steps[i]
             states.append(state)
+        if torch.cuda.is_current_stream_capturing() and not any(run.steps is t for t in self._captured):
+            self._captured.append(run.steps)  # the graph writes there as long as it lives, whatever becomes of the run
         grads = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in ps]
         adamw_step(ps, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], run.steps[at:end],
                    lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
@@ -185,10 +187,12 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ checkpoints
     def load_state_dict(self, state_dict) -> None:
         """Takes over a ``state_dict`` of this class, or one of ``torch.optim.AdamW`` (``Adam`` where it has no weight decay;
-        groups of a torch that does not say how its decay works are taken for AdamW's) with fp32 states where this optimizer's states are in 32 bits.  Groups that step by another rule -- ``maximize``,
-        ``amsgrad``, a weight decay that is added to the gradient, another class of optimizer -- are refused, and so are states
-        that do not fit; a refusal leaves this optimizer as it was.  (torch's own loading casts states to their parameter's
-        type, which would turn 8-bit codes and fp32 states of bf16 parameters into something else.)"""
+        groups of a torch that does not say how its decay works are taken for AdamW's) with fp32 states where this
+        optimizer's states are in 32 bits.  Groups that step by another rule -- ``maximize``, ``amsgrad``, a weight decay that
+        is added to the gradient, another class of optimizer -- are refused, and so are states that do not fit; a refusal
+        leaves this optimizer as it was.  The states are new tensors: a step captured before is captured again.  (torch's
+        own loading casts states to their parameter's type, which would turn 8-bit codes and fp32 states of bf16
+        parameters into something else.)"""
         saved = state_dict["param_groups"]
         for g in saved:
             self._refuse_another_rule(g)

@@ -167,3 +167,27 @@ def test_a_captured_step_goes_on_behind_a_count_that_was_set():
     pair.taken += 3
     pair.check("replayed")
     assert [int(pair.a.state[p]["step"]) for p in pair.ours] == [43] * 4
+
+
+def test_counts_that_a_graph_raises_outlive_a_change():
+    """A parameter that joins makes new arrays of step counts; a graph captured before goes on raising the old one, whose
+    memory belongs to nobody else."""
+    pair = Pair(8)
+    pair.step(2)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        pair.a.step()
+    counts = [int(pair.a.state[p]["step"]) for p in pair.ours]
+    more = torch.nn.Parameter(torch.zeros(50, device="cuda"))
+    pair.a.param_groups[0]["params"].append(more)
+    more.grad = torch.ones_like(more)
+    pair.a.step()
+    assert [int(pair.a.state[p]["step"]) for p in pair.ours] == [c + 1 for c in counts]
+    torch.cuda.synchronize()
+    small = [torch.zeros(2, dtype=torch.int32, device="cuda") for _ in range(2000)]     # takes what is free of that size
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert int(torch.stack(small).abs().sum()) == 0
+    assert [int(pair.a.state[p]["step"]) for p in pair.ours[:2]] == [c + 1 for c in counts[:2]]
